@@ -1,0 +1,229 @@
+// Causal depthwise convolution of packed rows with its state pages
+// (gdn_recoverssm_conv):
+//   out[t] = act(bias + sum_j w[j] x[t - taps + 1 + j]),
+// positions before a row's first token from its source page.
+//
+// A thread owns CH neighbouring channels over a tile of tokens and walks them
+// with the last taps - 1 inputs in registers, so each input is read once (and
+// taps - 1 of them again at a tile's start). Bound by reading x and writing
+// out. Whoever has a row's first token also writes its states, final and
+// boundary alike, from x: the only thread that reads the source page's
+// channels is the one that overwrites them, whatever pages coincide.
+#include "rows.cuh"
+
+namespace gdn {
+
+struct ConvArgs {
+  gdn_row_pages pages;
+  const void *x, *w, *bias;
+  void *out, *states;
+  int64_t x_ts, out_ts, bs, ds, ts;
+  int32_t D, tile, silu, groups;  // groups: workgroups over the channels
+};
+
+constexpr int kConvThreads = 256;
+
+// N consecutive elements, `live` of them inside the tensor.
+template <typename T, int N>
+__device__ __forceinline__ void load_live(const T *p, int live, float (&out)[N]) {
+  if (live == N) {
+    T raw[N];
+    __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = to_f32(raw[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = e < live ? to_f32(p[e]) : 0.0f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_live(T *p, int live, const float (&x)[N]) {
+  T raw[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) raw[e] = from_f32<T>(x[e]);
+  if (live == N) {
+    __builtin_memcpy(p, raw, sizeof(raw));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < live) p[e] = raw[e];
+  }
+}
+
+template <typename T, int TAPS, int CH>
+__global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
+  constexpr int HIST = TAPS - 1, U = 8;
+  const gdn_row_pages &p = a.pages;
+  const int d0 = (int(blockIdx.x % unsigned(a.groups)) * kConvThreads + int(threadIdx.x)) * CH;
+  const int live = a.D - d0 < CH ? a.D - d0 : CH;
+  int t = int(blockIdx.x / unsigned(a.groups)) * a.tile;
+  const int t1 = t + a.tile < p.tokens ? t + a.tile : int(p.tokens);
+  // Rows are found by whole waves; lanes past the channels leave after that.
+  int b = last_not_above(int(p.rows) + 1, t, [&](int i) {
+    return load_index(p.query_start_loc, i * p.qsl_stride, p.qsl_dtype);
+  });
+  b = __builtin_amdgcn_readfirstlane(b);
+  if (live <= 0) return;
+  float w[CH][TAPS], bias[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    float row[TAPS];
+    load_live<T, TAPS>(static_cast<const T *>(a.w) + int64_t(d0 + (c < live ? c : 0)) * TAPS, TAPS, row);
+#pragma unroll
+    for (int j = 0; j < TAPS; ++j) w[c][j] = row[j];
+    bias[c] = 0.0f;
+  }
+  if (a.bias) load_live<T, CH>(static_cast<const T *>(a.bias) + d0, live, bias);
+  const T *x = static_cast<const T *>(a.x) + d0;
+  T *out = static_cast<T *>(a.out) + d0;
+  if (b < 0) b = 0;
+  for (; t < t1 && b < p.rows; ++b) {
+    const Row r = load_row(p, b);
+    const int end = r.bos + r.n < t1 ? r.bos + r.n : t1;
+    if (r.n == 0 || end <= t) continue;
+    t = t < r.bos ? r.bos : t;
+    if (!r.valid) {
+      const float zero[CH] = {};
+      for (; t < end; ++t) store_live<T, CH>(out + t * a.out_ts, live, zero);
+      continue;
+    }
+    float h[HIST][CH];  // the inputs before t, oldest first
+    T *const states = static_cast<T *>(a.states);
+    const auto from_page = [&](int j, float (&to)[CH]) {
+      const T *s = states + r.src * a.bs + d0 * a.ds + j * a.ts;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) to[c] = !r.fresh && c < live ? to_f32(s[c * a.ds]) : 0.0f;
+    };
+#pragma unroll
+    for (int j = 0; j < HIST; ++j) {
+      const int at = t - r.bos - HIST + j;  // position in the row
+      if (at >= 0)
+        load_live<T, CH>(x + (r.bos + at) * a.x_ts, live, h[j]);
+      else
+        from_page(HIST + at, h[j]);
+    }
+    if (t == r.bos) {
+      // The states: the HIST inputs that end at position pos of the row, taken
+      // from the page's history (h, at this point) where pos < HIST.
+      const auto store_state = [&](int64_t page, int pos) {
+#pragma unroll
+        for (int j = 0; j < HIST; ++j) {
+          const int at = pos - HIST + j;
+          float in[CH];
+          if (at >= 0) {
+            load_live<T, CH>(x + (r.bos + at) * a.x_ts, live, in);
+          } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+              in[c] = 0.0f;
+#pragma unroll
+              for (int i = 0; i < HIST; ++i) in[c] = at + HIST == i ? h[i][c] : in[c];
+            }
+          }
+          T *s = states + page * a.bs + d0 * a.ds + j * a.ts;
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            if (c < live) s[c * a.ds] = from_f32<T>(in[c]);
+        }
+      };
+      if (p.block_table) {
+        for (int64_t pos = (r.C / p.block_size + 1) * p.block_size; pos < r.C + r.n; pos += p.block_size) {
+          const int64_t page = boundary_page(p, r, pos);
+          if (page != 0) store_state(page, int(pos - r.C));
+        }
+      }
+      store_state(r.fin, r.n);
+    }
+    while (t < end) {
+      const int m = end - t < U ? end - t : U;
+      float in[U][CH];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < m) load_live<T, CH>(x + int64_t(t + u) * a.x_ts, live, in[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u >= m) break;
+        float y[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          float s = bias[c];
+#pragma unroll
+          for (int j = 0; j < HIST; ++j) s = fmaf(w[c][j], h[j][c], s);
+          s = fmaf(w[c][HIST], in[u][c], s);
+          y[c] = a.silu ? s / (1.0f + expf(-s)) : s;
+#pragma unroll
+          for (int j = 0; j + 1 < HIST; ++j) h[j][c] = h[j + 1][c];
+          h[HIST - 1][c] = in[u][c];
+        }
+        store_live<T, CH>(out + int64_t(t + u) * a.out_ts, live, y);
+      }
+      t += m;
+    }
+  }
+}
+
+template <typename T, int CH>
+static void launch_conv(int taps, dim3 grid, hipStream_t s, const ConvArgs &a) {
+  switch (taps) {
+    case 2: hipLaunchKernelGGL((conv_kernel<T, 2, CH>), grid, dim3(kConvThreads), 0, s, a); break;
+    case 3: hipLaunchKernelGGL((conv_kernel<T, 3, CH>), grid, dim3(kConvThreads), 0, s, a); break;
+    case 4: hipLaunchKernelGGL((conv_kernel<T, 4, CH>), grid, dim3(kConvThreads), 0, s, a); break;
+    default: hipLaunchKernelGGL((conv_kernel<T, 5, CH>), grid, dim3(kConvThreads), 0, s, a); break;
+  }
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_recoverssm_conv(const gdn_conv_rows *l, void *stream) {
+  int status = GDN_OK;
+  if (!l) {
+    set_error("conv: missing launch");
+    return GDN_ERR_INVALID;
+  }
+  if (!check_row_pages("conv", l->pages, &status)) return status;
+  if (!float_type(l->dtype) || l->dim < 1 || l->dim > (1 << 24) || l->taps < 2 || l->taps > 5 ||
+      l->window < l->taps - 1) {
+    set_error("conv: dim=%lld taps=%lld window=%lld dtype=%d unsupported", (long long)l->dim, (long long)l->taps,
+              (long long)l->window, l->dtype);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (l->pages.rows == 0 || l->pages.tokens == 0) return GDN_OK;
+  if (!l->x || !l->weight || !l->out || !l->conv_states) {
+    set_error("conv: null tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  ConvArgs a{};
+  a.pages = l->pages;
+  a.x = l->x, a.w = l->weight, a.bias = l->bias, a.out = l->out, a.states = l->conv_states;
+  a.x_ts = l->x_stride, a.out_ts = l->out_stride;
+  a.bs = l->state_block_stride, a.ds = l->state_dim_stride, a.ts = l->state_token_stride;
+  a.D = int32_t(l->dim), a.silu = l->silu;
+  const bool wide = l->pages.tokens >= 8 * l->pages.rows;
+  a.tile = wide ? 32 : 1;
+  const int ch = wide ? 8 : 2;
+  a.groups = int32_t((l->dim + kConvThreads * ch - 1) / (kConvThreads * ch));
+  const int64_t blocks = (l->pages.tokens + a.tile - 1) / a.tile * a.groups;
+  if (blocks > 0x7fffffffLL) {
+    set_error("conv: grid too large");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  const dim3 grid = dim3(unsigned(blocks));
+  auto s = static_cast<hipStream_t>(stream);
+  if (wide) {
+    if (l->dtype == GDN_DT_BF16) launch_conv<bf16, 8>(int(l->taps), grid, s, a);
+    else if (l->dtype == GDN_DT_F16) launch_conv<f16, 8>(int(l->taps), grid, s, a);
+    else launch_conv<float, 8>(int(l->taps), grid, s, a);
+  } else {
+    if (l->dtype == GDN_DT_BF16) launch_conv<bf16, 2>(int(l->taps), grid, s, a);
+    else if (l->dtype == GDN_DT_F16) launch_conv<f16, 2>(int(l->taps), grid, s, a);
+    else launch_conv<float, 2>(int(l->taps), grid, s, a);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) {
+    set_error("conv: launch failed: %s", hipGetErrorString(err));
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}

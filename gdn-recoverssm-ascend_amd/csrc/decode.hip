@@ -1,0 +1,53 @@
+// C entry point of the recurrent gated delta rule.
+#include "decode_kernel.cuh"
+
+using namespace gdn;
+
+// Loads in flight per wave (NP rows of 1 KB each).
+static int decode_passes(int64_t rows, int64_t value_heads, int64_t V, int rows_per_load) {
+  const int64_t waves = rows * value_heads * ((V + 8 * rows_per_load - 1) / (8 * rows_per_load));
+  return waves < 2048 ? 2 : 8;
+}
+
+extern "C" int gdn_recoverssm_decode(const gdn_rule_launch *l, void *stream) {
+  int status = GDN_OK;
+  if (!check_rule("decode", l, &status)) return status;
+  if (l->pages.rows == 0 || l->pages.tokens == 0) return GDN_OK;
+  const int64_t K = l->key_dim, V = l->value_dim;
+  DecodeArgs a{};
+  a.pages = l->pages;
+  a.q = l->q, a.k = l->k, a.v = l->v, a.g = l->g, a.beta = l->beta, a.out = l->out, a.state = l->state;
+  a.a_log = l->a_log, a.dt_bias = l->dt_bias;
+  a.gated = l->gating != nullptr;
+  if (l->gating) a.gating = *l->gating;
+  a.q_ts = l->q_stride, a.k_ts = l->k_stride, a.v_ts = l->v_stride;
+  a.g_ts = l->g_stride, a.beta_ts = l->beta_stride, a.out_ts = l->out_stride;
+  a.state_bs = l->state_block_stride, a.state_hs = l->state_head_stride, a.state_vs = int32_t(l->state_v_stride);
+  a.K = int32_t(K), a.V = int32_t(V), a.HV = int32_t(l->value_heads);
+  a.ratio = uint32_t(l->value_heads / l->heads);
+  a.g_dt = l->g_dtype, a.beta_dt = l->beta_dtype;
+  a.out_f32 = l->out_dtype == GDN_DT_F32, a.l2norm = l->qk_l2norm, a.scale = l->scale;
+  const int base = l->state_dtype == GDN_DT_F32 ? 16 : 8;
+  const int lanes = K <= 64 ? base : K <= 128 ? 2 * base : 4 * base;
+  const int np = decode_passes(l->pages.rows, l->value_heads, V, 64 / lanes);
+  const int64_t tile_rows = int64_t(np) * (64 / lanes);
+  a.tiles = int32_t((V + tile_rows - 1) / tile_rows);
+  a.waves = l->pages.rows * l->value_heads * a.tiles;
+  const int64_t grid = (a.waves + kDecodeWaves - 1) / kDecodeWaves;
+  if (grid > 0x7fffffffLL) {
+    set_error("decode: grid too large");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  auto s = static_cast<hipStream_t>(stream);
+  switch (l->state_dtype) {
+    case GDN_DT_BF16: launch_decode<bf16>(l->act_dtype, lanes, np, unsigned(grid), s, a); break;
+    case GDN_DT_F16: launch_decode<f16>(l->act_dtype, lanes, np, unsigned(grid), s, a); break;
+    default: launch_decode<float>(l->act_dtype, lanes, np, unsigned(grid), s, a); break;
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) {
+    set_error("decode: launch failed: %s", hipGetErrorString(err));
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}

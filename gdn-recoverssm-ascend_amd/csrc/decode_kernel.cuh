@@ -1,0 +1,216 @@
+// Recurrent gated delta rule: every row's tokens one after the other with the
+// row's state in registers (gdn_recoverssm_decode).
+//
+// Per token, with d = e^g:  a = S k,  b = S q  (both from the state as it
+// stands),  c = beta (v - d a),  out = scale (d b + c (k.q)),
+// S <- d S + c k^T: one pass over the state, and the output needs no second
+// product because S_t q = d S_{t-1} q + c (k.q).
+//
+// A wave owns NP * (64 / LPR) rows of V of one (row, value head) state: LPR
+// lanes hold a state row (16 bytes each), NP loads are in flight per wave, and
+// sums over a row are butterflies over its lanes. No wave waits for another.
+// Bound by the page's read and write.
+#pragma once
+
+#include "rows.cuh"
+
+namespace gdn {
+
+struct DecodeArgs {
+  gdn_row_pages pages;
+  const void *q, *k, *v, *g, *beta, *a_log, *dt_bias;
+  void *out, *state;
+  gdn_gating_ext gating;
+  int64_t q_ts, k_ts, v_ts, g_ts, beta_ts, out_ts;
+  int64_t state_bs, state_hs;
+  int32_t state_vs;                 // elements
+  int32_t K, V, HV, tiles;          // tiles: per (row, value head)
+  uint32_t ratio;
+  int32_t g_dt, beta_dt, out_f32, gated, l2norm;
+  float scale;
+  int64_t waves;
+};
+
+constexpr int kDecodeWaves = 4;   // waves of a workgroup
+constexpr int kDecodeNT = 2;      // buffer cache policy: non-temporal
+constexpr int kDecodeOutside = 0x7ffff000;
+
+// E consecutive elements, aligned to an element only.
+template <typename A, int E>
+__device__ __forceinline__ void load_elems(const A *p, float (&out)[E]) {
+  A raw[E];
+  __builtin_memcpy(raw, p, sizeof(raw));
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[e] = to_f32(raw[e]);
+}
+
+template <typename S, typename A, int LPR, int NP>
+__global__ __launch_bounds__(64 * kDecodeWaves) void decode_kernel(const DecodeArgs a) {
+  constexpr int E = Chunk<S>::E, RPW = 64 / LPR;
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = int64_t(blockIdx.x) * kDecodeWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave >= a.waves) return;
+  const int tile = int(wave % a.tiles);
+  const int64_t rh = wave / a.tiles;
+  const int hv = int(rh % a.HV), b = int(rh / a.HV), h = int(uint32_t(hv) / a.ratio);
+  const Row r = load_row(a.pages, b);
+  if (r.n == 0) return;
+  const int v0 = tile * NP * RPW, group = lane / LPR, k0 = (lane % LPR) * E;
+  // The lane that stores pass p's result is the p-th of its group.
+  const int vmine = v0 + (lane % LPR) * RPW + group;
+  const bool stores = (lane % LPR) < NP && vmine < a.V;
+  const auto put = [&](int64_t tok, float x) {
+    const int64_t at = tok * a.out_ts + int64_t(hv) * a.V + vmine;
+    if (!stores) return;
+    if (a.out_f32)
+      static_cast<float *>(a.out)[at] = x;
+    else
+      static_cast<A *>(a.out)[at] = from_f32<A>(x);
+  };
+  if (!r.valid) {
+    for (int t = 0; t < r.n; ++t) put(r.bos + t, 0.0f);
+    return;
+  }
+  const int64_t row_bytes = int64_t(a.state_vs) * int64_t(sizeof(S));
+  const auto rsrc = [&](int64_t page) {
+    const S *base = static_cast<const S *>(a.state) + page * a.state_bs + hv * a.state_hs;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(base), 0, 0x7fff0000, 0x00020000);
+  };
+  const bool klive = k0 < a.K;
+  int off[NP];
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const int v = v0 + p * RPW + group;
+    off[p] = klive && v < a.V ? int(v * row_bytes) + k0 * int(sizeof(S)) : kDecodeOutside;
+  }
+  float s[NP][E];
+  if (r.fresh) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[p][e] = 0.0f;
+  } else {
+    const auto src = rsrc(r.src);
+    uint4 raw[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const auto u = __builtin_amdgcn_raw_buffer_load_b128(src, off[p], 0, kDecodeNT);
+      raw[p] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) unpack16<S>(raw[p], s[p]);
+  }
+  const auto store_state = [&](int64_t page) {
+    const auto dst = rsrc(page);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const uint4 u = pack16<S>(s[p]);
+      store_b128_settled<kDecodeNT>(gdn_u32x4{u.x, u.y, u.z, u.w}, dst, off[p], 0);
+    }
+  };
+  const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
+  const int kat = klive ? k0 : 0;  // lanes past K read the row's first elements and drop them
+  for (int t = 0; t < r.n; ++t) {
+    const int64_t tok = r.bos + t;
+    float k[E], q[E], v[NP];
+    load_elems(static_cast<const A *>(a.k) + tok * a.k_ts + int64_t(h) * a.K + kat, k);
+    load_elems(static_cast<const A *>(a.q) + tok * a.q_ts + int64_t(h) * a.K + kat, q);
+    const A *vp = static_cast<const A *>(a.v) + tok * a.v_ts + int64_t(hv) * a.V;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int row = v0 + p * RPW + group;
+      v[p] = to_f32(vp[row < a.V ? row : a.V - 1]);
+    }
+    const float d = expf(log_decay(gates, load_as_f32(a.g, tok * a.g_ts + hv, a.g_dt)));
+    const float beta = beta_of(gates, load_as_f32(a.beta, tok * a.beta_ts + hv, a.beta_dt));
+    float kq = 0.0f, kk = 0.0f, qq = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      k[e] = klive ? k[e] : 0.0f;
+      q[e] = klive ? q[e] : 0.0f;
+    }
+    if (a.l2norm) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        kk = fmaf(k[e], k[e], kk);
+        qq = fmaf(q[e], q[e], qq);
+      }
+      const float rk = 1.0f / sqrtf(group_sum<LPR>(kk) + 1e-6f), rq = 1.0f / sqrtf(group_sum<LPR>(qq) + 1e-6f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        k[e] *= rk;
+        q[e] *= rq;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      q[e] *= a.scale;
+      kq = fmaf(k[e], q[e], kq);
+    }
+    kq = group_sum<LPR>(kq);
+    float mine = 0.0f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      float sk = 0.0f, sq = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s[p][e] *= d;
+        sk = fmaf(s[p][e], k[e], sk);
+        sq = fmaf(s[p][e], q[e], sq);
+      }
+      sk = group_sum<LPR>(sk);
+      sq = group_sum<LPR>(sq);
+      const float c = beta * (v[p] - sk);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[p][e] = fmaf(c, k[e], s[p][e]);
+      const float o = fmaf(c, kq, sq);
+      mine = lane % LPR == p ? o : mine;
+    }
+    put(tok, mine);
+    if (a.pages.block_table && t + 1 < r.n) {
+      const int64_t page = boundary_page(a.pages, r, r.C + t + 1);
+      if (page != 0) store_state(page);
+    }
+  }
+  store_state(r.fin);
+}
+
+// NP by rule (see gdn_recoverssm_decode), LPR by K.
+template <typename S, typename A, int LPR>
+static void launch_decode_lanes(int np, unsigned grid, hipStream_t s, const DecodeArgs &a) {
+  if (np == 2)
+    hipLaunchKernelGGL((decode_kernel<S, A, LPR, 2>), dim3(grid), dim3(64 * kDecodeWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((decode_kernel<S, A, LPR, 8>), dim3(grid), dim3(64 * kDecodeWaves), 0, s, a);
+}
+template <typename S, typename A>
+static void launch_decode_act(int lanes, int np, unsigned grid, hipStream_t s, const DecodeArgs &a) {
+  constexpr int L = sizeof(S) == 4 ? 16 : 8;  // lanes of a row of K <= 64
+  if (lanes == L)
+    launch_decode_lanes<S, A, L>(np, grid, s, a);
+  else if (lanes == 2 * L)
+    launch_decode_lanes<S, A, 2 * L>(np, grid, s, a);
+  else
+    launch_decode_lanes<S, A, 4 * L>(np, grid, s, a);
+}
+template <typename S>
+void launch_decode(int act, int lanes, int np, unsigned grid, hipStream_t s, const DecodeArgs &a);
+
+#define GDN_DECODE_STATE(S)                                                                              \
+  template <>                                                                                            \
+  void launch_decode<S>(int act, int lanes, int np, unsigned grid, hipStream_t s, const DecodeArgs &a) { \
+    if (act == GDN_DT_BF16)                                                                              \
+      launch_decode_act<S, bf16>(lanes, np, grid, s, a);                                                 \
+    else if (act == GDN_DT_F16)                                                                          \
+      launch_decode_act<S, f16>(lanes, np, grid, s, a);                                                  \
+    else                                                                                                 \
+      launch_decode_act<S, float>(lanes, np, grid, s, a);                                                \
+  }
+template <>
+void launch_decode<float>(int, int, int, unsigned, hipStream_t, const DecodeArgs &);
+template <>
+void launch_decode<bf16>(int, int, int, unsigned, hipStream_t, const DecodeArgs &);
+template <>
+void launch_decode<f16>(int, int, int, unsigned, hipStream_t, const DecodeArgs &);
+
+}  // namespace gdn

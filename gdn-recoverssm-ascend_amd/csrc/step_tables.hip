@@ -1,0 +1,276 @@
+// A step's tables from its rows' lengths (gdn_recoverssm_step_tables) and the
+// return of pages to the ring of free ones (gdn_recoverssm_release_pages).
+//
+// Every workgroup sums the lengths and the page needs of all rows for itself
+// (two prefix sums over at most 4096 rows, held in LDS) and then fills its own
+// tile of tokens: no workgroup waits for another, so the step is one launch.
+// A token of a newly taken block finds its page in the ring by the row's
+// prefix, whether or not the table's entry has been written yet; the entry is
+// written by the token that starts the block (every new block has one). Bound
+// by latency: the lengths' round trip, the scan, the pages' round trip.
+#include "rows.cuh"
+
+namespace gdn {
+
+constexpr int kTableThreads = 256;
+constexpr int kTableTile = 1024;  // tokens of a workgroup
+
+struct TableRow {
+  int64_t C;
+  int n, need;  // new tokens, new pages
+  int64_t req;
+  bool known;
+};
+
+__device__ __forceinline__ TableRow table_row(const gdn_step_tables &a, int r) {
+  TableRow t;
+  t.req = a.request_indices ? load_index(a.request_indices, r * a.map_stride, a.map_dtype) : r;
+  t.known = t.req >= 0 && t.req < a.table_rows && t.req < a.computed_len;
+  t.C = t.known ? load_index(a.num_computed, t.req * a.computed_stride, a.computed_dtype) : 0;
+  const int64_t n = load_index(a.query_lens, r * a.lens_stride, a.lens_dtype);
+  t.C = t.C < 0 ? 0 : t.C;
+  t.n = int(n < 0 ? 0 : n > 0x3fffffff ? 0x3fffffff : n);
+  const int64_t have = (t.C + a.block_size - 1) / a.block_size, all = (t.C + t.n + a.block_size - 1) / a.block_size;
+  t.known = t.known && all <= a.table_width;
+  t.need = t.known ? int(all - have) : 0;
+  return t;
+}
+
+__device__ __forceinline__ int ring_page(const gdn_step_tables &a, int64_t place) {
+  const int64_t i = place % a.free_len;
+  return a.free_pages[i < 0 ? i + a.free_len : i];
+}
+
+__global__ __launch_bounds__(kTableThreads) void step_tables_kernel(const gdn_step_tables a) {
+  extern __shared__ int sums[];  // token starts [rows + 1], then page starts [rows + 1]
+  __shared__ int64_t wave_sum[kTableThreads / 64];
+  const int rows = int(a.rows), tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  int *const starts = sums, *const pages = sums + rows + 1;
+  // Each thread sums a run of rows, the workgroup scans the runs. Tokens and
+  // pages share one 64-bit sum: tokens saturate below 2^31, pages are fewer.
+  const int per = (rows + kTableThreads - 1) / kTableThreads, r0 = tid * per;
+  const int r1 = r0 + per < rows ? r0 + per : rows;
+  uint64_t mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const TableRow t = table_row(a, r);
+    starts[r] = t.n;
+    pages[r] = t.need;
+    mine += (uint64_t(uint32_t(t.need)) << 32) + uint32_t(t.n);
+  }
+  uint64_t run = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t o = __shfl_up(run, d);
+    run += lane >= d ? o : 0;
+  }
+  if (lane == 63) wave_sum[wv] = int64_t(run);
+  __syncthreads();
+  uint64_t before = run - mine;
+  for (int w = 0; w < wv; ++w) before += uint64_t(wave_sum[w]);
+  for (int r = r0; r < r1; ++r) {
+    const uint32_t n = uint32_t(starts[r]), need = uint32_t(pages[r]);
+    starts[r] = int(uint32_t(before));
+    pages[r] = int(before >> 32);
+    before += (uint64_t(need) << 32) + n;
+  }
+  if (tid == 0) {
+    uint64_t all = 0;
+    for (int w = 0; w < kTableThreads / 64; ++w) all += uint64_t(wave_sum[w]);
+    starts[rows] = int(uint32_t(all));
+    pages[rows] = int(all >> 32);
+  }
+  __syncthreads();
+  const int64_t head = a.free_span[0], tail = a.free_span[1];
+  int64_t room = tail - head;
+  room = room < 0 ? 0 : room > a.free_len ? a.free_len : room;
+  // A row is served if it needs no page or its pages and all before it fit.
+  const auto served = [&](int r) { return pages[r + 1] == pages[r] || pages[r + 1] <= room; };
+
+  // Tokens of this workgroup's tile.
+  const int64_t t0 = int64_t(blockIdx.x) * kTableTile;
+  for (int i = tid; i < kTableTile; i += kTableThreads) {
+    const int64_t t = t0 + i;
+    if (t >= a.num_tokens) break;
+    int64_t pos = -1, slot = -1;
+    if (t < starts[rows]) {
+      int lo = 0, hi = rows;  // the last row that starts at or before t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int r = lo;
+      const TableRow row = table_row(a, r);
+      pos = row.C + (t - starts[r]);
+      if (row.known && served(r)) {
+        const int64_t col = pos / a.block_size, in = pos % a.block_size;
+        const int64_t have = (row.C + a.block_size - 1) / a.block_size;
+        int32_t *entry = a.block_table + row.req * a.table_row_stride + col;
+        int page;
+        if (col >= have) {
+          page = ring_page(a, head + pages[r] + (col - have));
+          if (in == 0) *entry = page;
+        } else {
+          page = *entry;
+        }
+        slot = int64_t(page) * a.block_size + in;
+      }
+    }
+    a.positions[t] = pos;
+    a.slot_mapping[t] = slot;
+  }
+  // Rows, spread over the workgroups.
+  for (int r = blockIdx.x * kTableThreads + tid; r < rows; r += gridDim.x * kTableThreads) {
+    const TableRow row = table_row(a, r);
+    const bool ok = row.known && served(r);
+    const int64_t seq = row.C + row.n, have = (row.C + a.block_size - 1) / a.block_size;
+    const int32_t *entries = a.block_table + row.req * a.table_row_stride;
+    int source = 0, last = 0;
+    if (row.known && row.C > 0) source = entries[(row.C - 1) / a.block_size];
+    if (ok && seq > 0) {
+      const int64_t col = (seq - 1) / a.block_size;
+      last = col >= have ? ring_page(a, head + pages[r] + (col - have)) : entries[col];
+    }
+    a.query_start_loc[r] = starts[r];
+    a.seq_lens[r] = int(seq < 0x7fffffff ? seq : 0x7fffffff);
+    a.source_indices[r] = source;
+    a.final_indices[r] = last;
+    a.new_pages[r] = ok ? row.need : -1;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.query_start_loc[rows] = starts[rows];
+    // Served rows take a prefix of the needs: the last row whose pages fit.
+    int lo = 0, hi = rows + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pages[mid] <= room) lo = mid;
+      else hi = mid;
+    }
+    a.free_span_out[0] = head + pages[lo];
+    a.free_span_out[1] = tail;
+  }
+}
+
+struct ReleaseArgs {
+  const void *requests, *lens;
+  int32_t requests_dt, lens_dt;
+  int64_t count, lens_stride;
+  int32_t *table;
+  int64_t table_rows, table_width, table_row_stride, block;
+  int32_t *free_pages;
+  int64_t free_len;
+  const int64_t *span;
+  int64_t *span_out;
+};
+
+// One workgroup: ended requests are few, and the ring's order is that of the
+// list. Per request, runs of 256 columns: a ballot counts the pages before a
+// lane's own.
+__global__ __launch_bounds__(kTableThreads) void release_pages_kernel(const ReleaseArgs a) {
+  __shared__ int counts[kTableThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t head = a.span[0];
+  int64_t tail = a.span[1];
+  for (int64_t i = 0; i < a.count; ++i) {
+    const int64_t req = load_index(a.requests, i, a.requests_dt);
+    if (req < 0 || req >= a.table_rows) continue;
+    int64_t cols = load_index(a.lens, i * a.lens_stride, a.lens_dt);
+    cols = cols <= 0 ? 0 : (cols - 1) / a.block + 1;
+    cols = cols < a.table_width ? cols : a.table_width;
+    int32_t *row = a.table + req * a.table_row_stride;
+    for (int64_t c0 = 0; c0 < cols; c0 += kTableThreads) {
+      const int64_t c = c0 + tid;
+      const int page = c < cols ? row[c] : 0;
+      const uint64_t some = __builtin_amdgcn_ballot_w64(page != 0);
+      if (lane == 0) counts[wv] = __popcll(some);
+      __syncthreads();
+      int before = __popcll(some & ((uint64_t(1) << lane) - 1)), all = 0;
+#pragma unroll
+      for (int w = 0; w < kTableThreads / 64; ++w) {
+        before += w < wv ? counts[w] : 0;
+        all += counts[w];
+      }
+      const int64_t place = tail + before;
+      if (page != 0 && place - head < a.free_len) a.free_pages[((place % a.free_len) + a.free_len) % a.free_len] = page;
+      if (c < cols) row[c] = 0;
+      tail = tail + all - head < a.free_len ? tail + all : head + a.free_len;
+      __syncthreads();
+    }
+  }
+  if (tid == 0) {
+    a.span_out[0] = head;
+    a.span_out[1] = tail;
+  }
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_recoverssm_step_tables(const gdn_step_tables *l, void *stream) {
+  if (!l) {
+    set_error("step_tables: missing launch");
+    return GDN_ERR_INVALID;
+  }
+  if (l->rows < 0 || l->rows > GDN_TABLES_MAX_ROWS || l->num_tokens < 0 || l->num_tokens > 0x3fffffff ||
+      l->table_width < 1 || l->table_rows < 0 || l->free_len < 1 || l->block_size < 1 || l->computed_len < 0) {
+    set_error("step_tables: rows=%lld (at most %d) tokens=%lld width=%lld ring=%lld block=%lld", (long long)l->rows,
+              GDN_TABLES_MAX_ROWS, (long long)l->num_tokens, (long long)l->table_width, (long long)l->free_len,
+              (long long)l->block_size);
+    return GDN_ERR_INVALID;
+  }
+  if (!index_type(l->computed_dtype) || !index_type(l->lens_dtype) ||
+      (l->request_indices && !index_type(l->map_dtype))) {
+    set_error("step_tables: lengths and request indices must be int32 or int64");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (!l->free_pages || !l->free_span || !l->free_span_out || !l->query_start_loc ||
+      (l->num_tokens > 0 && (!l->positions || !l->slot_mapping)) ||
+      (l->rows > 0 && (!l->num_computed || !l->query_lens || !l->block_table || !l->seq_lens || !l->source_indices ||
+                       !l->final_indices || !l->new_pages))) {
+    set_error("step_tables: null pointer");
+    return GDN_ERR_INVALID;
+  }
+  if (l->free_span == l->free_span_out) {
+    set_error("step_tables: free_span_out must not be free_span");
+    return GDN_ERR_INVALID;
+  }
+  const int64_t tiles = (l->num_tokens + kTableTile - 1) / kTableTile;
+  const unsigned grid = unsigned(tiles > 1 ? tiles : 1);
+  hipLaunchKernelGGL(step_tables_kernel, dim3(grid), dim3(kTableThreads), unsigned(2 * (l->rows + 1) * 4),
+                     static_cast<hipStream_t>(stream), *l);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) {
+    set_error("step_tables: launch failed: %s", hipGetErrorString(err));
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}
+
+extern "C" int gdn_recoverssm_release_pages(const void *requests, int32_t requests_dtype, int64_t num_requests,
+                                            const void *seq_lens, int32_t lens_dtype, int64_t lens_stride,
+                                            int32_t *block_table, int64_t table_rows, int64_t table_width,
+                                            int64_t table_row_stride, int64_t block_size, int32_t *free_pages,
+                                            int64_t free_len, const int64_t *free_span, int64_t *free_span_out,
+                                            void *stream) {
+  if (num_requests < 0 || table_rows < 0 || table_width < 1 || block_size < 1 || free_len < 1 || !free_pages ||
+      !free_span || !free_span_out || free_span == free_span_out ||
+      (num_requests > 0 && (!requests || !seq_lens || !block_table))) {
+    set_error("release_pages: requests=%lld width=%lld block=%lld ring=%lld, or a missing pointer",
+              (long long)num_requests, (long long)table_width, (long long)block_size, (long long)free_len);
+    return GDN_ERR_INVALID;
+  }
+  if (!index_type(requests_dtype) || !index_type(lens_dtype)) {
+    set_error("release_pages: requests and lengths must be int32 or int64");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  ReleaseArgs a{requests, seq_lens, requests_dtype, lens_dtype, num_requests, lens_stride, block_table, table_rows,
+                table_width, table_row_stride, block_size, free_pages, free_len, free_span, free_span_out};
+  hipLaunchKernelGGL(release_pages_kernel, dim3(1), dim3(kTableThreads), 0, static_cast<hipStream_t>(stream), a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess) {
+    set_error("release_pages: launch failed: %s", hipGetErrorString(err));
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}

@@ -28,6 +28,18 @@ from .kernels import (  # noqa: F401
     record_geometry_bytes,
     record_nbytes,
 )
+from .prompt import (  # noqa: F401
+    gdn_recoverssm_conv,
+    gdn_recoverssm_decode,
+    gdn_recoverssm_decode_gated,
+    gdn_recoverssm_prefill,
+    gdn_recoverssm_prefill_gated,
+)
+from .step_tables import (  # noqa: F401
+    StepTables,
+    gdn_recoverssm_release_pages,
+    gdn_recoverssm_step_tables,
+)
 
 
 def initialize():
@@ -68,8 +80,16 @@ __all__ = [
     "NULL_BLOCK_ID",
     "PendingCommit",
     "ReplayRecordBuffers",
+    "StepTables",
     "continue_pending",
     "counts",
+    "gdn_recoverssm_conv",
+    "gdn_recoverssm_decode",
+    "gdn_recoverssm_decode_gated",
+    "gdn_recoverssm_prefill",
+    "gdn_recoverssm_prefill_gated",
+    "gdn_recoverssm_release_pages",
+    "gdn_recoverssm_step_tables",
     "gdn_recoverssm_verify",
     "gdn_recoverssm_verify_deferred",
     "gdn_recoverssm_verify_gated",

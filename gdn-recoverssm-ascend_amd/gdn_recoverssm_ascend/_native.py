@@ -154,6 +154,56 @@ class ConvLaunch(ctypes.Structure):  # gdn_conv_launch: the conv tables of gdn_r
 NOALLOC_PLAN_ENTRIES = 32768  # GDN_NOALLOC_PLAN_ENTRIES
 
 
+class RowPages(ctypes.Structure):  # gdn_row_pages
+    _fields_ = [
+        ("query_start_loc", c_vp), ("state_indices", c_vp), ("final_indices", c_vp), ("num_computed", c_vp),
+        ("block_table", c_vp), ("request_indices", c_vp),
+        ("rows", c_i64), ("tokens", c_i64), ("blocks", c_i64),
+        ("qsl_stride", c_i64), ("si_stride", c_i64), ("final_stride", c_i64), ("computed_stride", c_i64),
+        ("map_stride", c_i64), ("computed_len", c_i64),
+        ("table_row_stride", c_i64), ("table_col_stride", c_i64), ("table_rows", c_i64), ("table_width", c_i64),
+        ("block_size", c_i64),
+        ("qsl_dtype", c_i32), ("si_dtype", c_i32), ("final_dtype", c_i32), ("computed_dtype", c_i32),
+        ("map_dtype", c_i32), ("table_dtype", c_i32),
+    ]
+
+
+class RuleLaunch(ctypes.Structure):  # gdn_rule_launch
+    _fields_ = [
+        ("pages", RowPages),
+        ("q", c_vp), ("k", c_vp), ("v", c_vp), ("g", c_vp), ("beta", c_vp), ("out", c_vp), ("state", c_vp),
+        ("a_log", c_vp), ("dt_bias", c_vp), ("gating", ctypes.POINTER(GatingExt)),
+        ("heads", c_i64), ("value_heads", c_i64), ("key_dim", c_i64), ("value_dim", c_i64),
+        ("q_stride", c_i64), ("k_stride", c_i64), ("v_stride", c_i64), ("g_stride", c_i64), ("beta_stride", c_i64),
+        ("out_stride", c_i64), ("state_block_stride", c_i64), ("state_head_stride", c_i64), ("state_v_stride", c_i64),
+        ("act_dtype", c_i32), ("g_dtype", c_i32), ("beta_dtype", c_i32), ("out_dtype", c_i32), ("state_dtype", c_i32),
+        ("qk_l2norm", c_i32), ("scale", ctypes.c_float), ("reserved", c_i32),
+    ]
+
+
+class ConvRows(ctypes.Structure):  # gdn_conv_rows
+    _fields_ = [
+        ("pages", RowPages),
+        ("x", c_vp), ("weight", c_vp), ("bias", c_vp), ("out", c_vp), ("conv_states", c_vp),
+        ("dim", c_i64), ("taps", c_i64), ("window", c_i64), ("x_stride", c_i64), ("out_stride", c_i64),
+        ("state_block_stride", c_i64), ("state_dim_stride", c_i64), ("state_token_stride", c_i64),
+        ("dtype", c_i32), ("silu", c_i32),
+    ]
+
+
+class StepTablesLaunch(ctypes.Structure):  # gdn_step_tables
+    _fields_ = [
+        ("num_computed", c_vp), ("query_lens", c_vp), ("request_indices", c_vp), ("block_table", c_vp),
+        ("free_pages", c_vp), ("free_span", c_vp), ("free_span_out", c_vp),
+        ("query_start_loc", c_vp), ("seq_lens", c_vp), ("source_indices", c_vp), ("final_indices", c_vp),
+        ("new_pages", c_vp), ("positions", c_vp), ("slot_mapping", c_vp),
+        ("rows", c_i64), ("num_tokens", c_i64), ("computed_len", c_i64), ("computed_stride", c_i64),
+        ("lens_stride", c_i64), ("map_stride", c_i64), ("table_rows", c_i64), ("table_width", c_i64),
+        ("table_row_stride", c_i64), ("free_len", c_i64), ("block_size", c_i64),
+        ("computed_dtype", c_i32), ("lens_dtype", c_i32), ("map_dtype", c_i32), ("reserved", c_i32),
+    ]
+
+
 def plan_launch(plan_args: tuple) -> PlanLaunch:
     """The gdn_recoverssm_plan argument tuple (without the stream) as a PlanLaunch."""
     (sampled, sampled_dtype, sampled_stride, sampled_len, groups, num_groups, source, lens, final, boundary,
@@ -242,6 +292,19 @@ def load() -> ctypes.CDLL:
         lib.gdn_recoverssm_settle.restype = ctypes.c_int
         lib.gdn_recoverssm_settle.argtypes = [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64,
                                               ctypes.POINTER(SettleNext), c_vp, c_vp, c_vp, c_vp]
+        rule = ctypes.POINTER(RuleLaunch)
+        for name, args in (
+            ("decode", [rule, c_vp]),
+            ("prefill", [rule, c_vp, c_i64, c_vp]),
+            ("conv", [ctypes.POINTER(ConvRows), c_vp]),
+            ("step_tables", [ctypes.POINTER(StepTablesLaunch), c_vp]),
+            ("release_pages", [c_vp, c_i32, c_i64, c_vp, c_i32, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64,
+                               c_vp, c_vp, c_vp]),
+        ):
+            fn = getattr(lib, "gdn_recoverssm_" + name)
+            fn.restype, fn.argtypes = ctypes.c_int, args
+        lib.gdn_recoverssm_prefill_workspace.restype = c_i64
+        lib.gdn_recoverssm_prefill_workspace.argtypes = [rule]
         version = lib.gdn_recoverssm_abi_version()
         if version != ABI_VERSION:
             raise RuntimeError(f"GDN RecoverSSM HIP library ABI mismatch: {version} != {ABI_VERSION}")
@@ -282,6 +345,12 @@ def exported_symbols() -> tuple[str, ...]:
         "gdn_recoverssm_publish",
         "gdn_recoverssm_set_state_cache_retain",
         "gdn_recoverssm_settle",
+        "gdn_recoverssm_decode",
+        "gdn_recoverssm_prefill",
+        "gdn_recoverssm_prefill_workspace",
+        "gdn_recoverssm_conv",
+        "gdn_recoverssm_step_tables",
+        "gdn_recoverssm_release_pages",
     )
 
 

@@ -1,0 +1,389 @@
+"""The prompt and the plain decode of a Gated DeltaNet layer.
+
+No counterpart in the reference, which leaves both to its host framework: these
+make the state pages that the speculative verify and commit go on from, and
+carry requests that decode without drafts.
+
+* ``gdn_recoverssm_prefill`` / ``gdn_recoverssm_prefill_gated``: the gated delta
+  rule over packed prompts, a chunk of tokens at a time on the matrix cores;
+* ``gdn_recoverssm_decode`` / ``gdn_recoverssm_decode_gated``: the same rule
+  token by token, for rows of one or a few tokens;
+* ``gdn_recoverssm_conv``: the layer's causal depthwise convolution over the
+  same rows, with its state pages.
+
+All take a batch of rows packed along the tokens and describe it alike:
+
+* ``query_start_loc`` [B + 1]: row b's tokens (a row may have none);
+* ``state_indices`` [B]: the page its state starts from;
+* ``final_indices`` [B]: the page it ends in (default: the page it starts from);
+* ``num_computed`` (by request): the tokens C that came before; a row with C = 0
+  starts from a zero state, whatever its page holds (default: every row
+  continues from its page);
+* ``block_table`` [requests, W] with ``block_size`` (prefix-cache align mode,
+  instead of ``final_indices``; needs ``num_computed``): the row ends in the
+  page of column (C + n - 1) // block_size, and the state at every block
+  boundary inside the row goes to that boundary's page, column
+  boundary // block_size - 1, unless that entry is the null page;
+* ``request_indices`` [B]: row b's request in ``num_computed`` and
+  ``block_table`` (default: request b).
+
+A page <= 0 or past the pool is the null page: a row that ends in one, or has to
+start from one, gives zero outputs and stores nothing. Pages of different rows
+must not coincide. Integer arrays are int32 or int64, of any stride.
+
+Arguments are checked before anything is launched (``ValueError("GDN
+RecoverSSM: ...")``); launches go on the current stream without synchronising.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as N
+from ._rules import enforce, fail
+from .kernels import _COUNTS, _FLOAT_TYPES, _INDEX_TYPES, MAX_KEY_DIM
+
+_ROW_RULES = (
+    ("query_start_loc must be one-dimensional with one entry more than state_indices",
+     lambda p: p[0].ndim == 1 and p[1].ndim == 1 and p[0].shape[0] == p[1].shape[0] + 1),
+    ("final_indices must have one entry per row",
+     lambda p: p[2] is None or (p[2].ndim == 1 and p[2].shape[0] == p[1].shape[0])),
+    ("num_computed must be one-dimensional", lambda p: p[3] is None or p[3].ndim == 1),
+    ("request_indices must have one entry per row",
+     lambda p: p[5] is None or (p[5].ndim == 1 and p[5].shape[0] == p[1].shape[0])),
+    ("num_computed needs one entry per row when there are no request_indices",
+     lambda p: p[3] is None or p[5] is not None or p[3].shape[0] >= p[1].shape[0]),
+    ("a block table takes the place of final_indices and needs num_computed and a positive block_size",
+     lambda p: p[4] is None or (p[2] is None and p[3] is not None and p[6] is not None and p[6] > 0)),
+    ("block_size comes with a block table", lambda p: p[4] is not None or p[6] is None),
+    ("the block table must be two-dimensional with at least one column",
+     lambda p: p[4] is None or (p[4].ndim == 2 and p[4].shape[1] > 0)),
+    ("offsets, indices, lengths and the block table must be int32 or int64",
+     lambda p: all(t is None or t.dtype in _INDEX_TYPES for t in p[:6])),
+)
+
+
+def _row_pages(parts: tuple, tokens: int, blocks: int, device) -> N.RowPages:
+    """The rows' description, checked, as the C ABI takes it; ``parts`` are
+    (query_start_loc, state_indices, final_indices, num_computed, block_table,
+    request_indices, block_size)."""
+    enforce(_ROW_RULES, parts)
+    if any(t is not None and t.device != device for t in parts[:6]):
+        fail("inputs must be on the same device")
+    qsl, source, final, computed, table, requests, block = parts
+    p = N.RowPages(qsl.data_ptr(), source.data_ptr())
+    p.rows, p.tokens, p.blocks = source.shape[0], tokens, blocks
+    p.qsl_stride, p.qsl_dtype = qsl.stride(0), N.dtype_code(qsl.dtype)
+    p.si_stride, p.si_dtype = source.stride(0), N.dtype_code(source.dtype)
+    if final is not None:
+        p.final_indices, p.final_stride, p.final_dtype = final.data_ptr(), final.stride(0), N.dtype_code(final.dtype)
+    if computed is not None:
+        p.num_computed, p.computed_len = computed.data_ptr(), computed.shape[0]
+        p.computed_stride, p.computed_dtype = computed.stride(0), N.dtype_code(computed.dtype)
+    if requests is not None:
+        p.request_indices, p.map_stride = requests.data_ptr(), requests.stride(0)
+        p.map_dtype = N.dtype_code(requests.dtype)
+    if table is not None:
+        p.block_table, p.table_dtype, p.block_size = table.data_ptr(), N.dtype_code(table.dtype), block
+        p.table_rows, p.table_width = table.shape
+        p.table_row_stride, p.table_col_stride = table.stride()
+    return p
+
+
+_RULE_RULES = (
+    ("q must have shape [1, tokens, heads, dim]", lambda c: c.q.ndim == 4 and c.q.shape[0] == 1),
+    ("q and k shapes differ", lambda c: c.k.shape == c.q.shape),
+    ("v must have shape [1, tokens, value heads, dim]",
+     lambda c: c.v.ndim == 4 and c.v.shape[0] == 1 and c.v.shape[1] == c.q.shape[1]),
+    ("value heads must be a positive multiple of the q/k heads",
+     lambda c: 0 < c.q.shape[2] <= c.v.shape[2] and c.v.shape[2] % c.q.shape[2] == 0),
+    ("q, k and v heads must be contiguous",
+     lambda c: all(t.stride(3) == 1 and t.stride(2) == t.shape[3] for t in (c.q, c.k, c.v))),
+    ("q, k and v must share one activation dtype (FP32, BF16 or FP16)",
+     lambda c: c.q.dtype == c.k.dtype == c.v.dtype and c.q.dtype in _FLOAT_TYPES),
+    ("gate or beta shape is incompatible", lambda c: all(t.numel() == c.v.shape[1] * c.v.shape[2] for t in (c.g, c.beta))),
+    ("gate and beta must be FP32 or the activation dtype",
+     lambda c: all(t.dtype in (torch.float32, c.q.dtype) for t in (c.g, c.beta))),
+    ("checkpoint must be four-dimensional", lambda c: c.state.ndim == 4),
+    ("checkpoint shape is incompatible",
+     lambda c: tuple(c.state.shape[1:]) == (c.v.shape[2], c.v.shape[3], c.q.shape[3]) and c.state.shape[0] > 0),
+    ("checkpoint dtype is not supported", lambda c: c.state.dtype in _FLOAT_TYPES),
+    (f"checkpoint rows must be contiguous, 16-byte aligned and K <= {MAX_KEY_DIM} a multiple of 16 bytes",
+     lambda c: c.q.shape[3] <= MAX_KEY_DIM and c.state.stride(3) == 1 and c.state.data_ptr() % 16 == 0
+     and all(s * c.state.element_size() % 16 == 0 for s in (c.q.shape[3], *c.state.stride()[:3]))),
+    ("output shape or layout is incompatible",
+     lambda c: c.out.shape == c.v.shape and c.out.stride(3) == 1 and c.out.stride(2) == c.v.shape[3]),
+    ("out must be FP32 or the activation dtype", lambda c: c.out.dtype in (torch.float32, c.q.dtype)),
+    ("A_log and dt_bias need one contiguous entry per value head",
+     lambda c: c.a_log is None or all(t.ndim == 1 and t.shape[0] == c.v.shape[2] and t.stride(0) == 1
+                                      and t.dtype in _FLOAT_TYPES for t in (c.a_log, c.dt_bias))),
+    ("softplus beta must be positive", lambda c: c.a_log is None or c.softplus[0] > 0.0),
+    ("inputs must be on the same device",
+     lambda c: all(t is None or t.device == c.q.device
+                   for t in (c.k, c.v, c.g, c.beta, c.state, c.out, c.a_log, c.dt_bias))),
+    ("prefill and decode run on a HIP device", lambda c: c.q.device.type == "cuda"),
+)
+
+
+class _RuleCall:
+    """One call of the rule: its tensors, and the launch that follows."""
+
+    def __init__(self, g, beta, q, k, v, state, out, a_log=None, dt_bias=None, softplus=(1.0, 20.0)):
+        self.g, self.beta, self.q, self.k, self.v, self.state = g, beta, q, k, v, state
+        self.out = torch.empty(v.shape, dtype=v.dtype, device=v.device) if out is None else out
+        self.a_log, self.dt_bias, self.softplus = a_log, dt_bias, softplus
+
+    def launch(self, parts, scale, normalized) -> N.RuleLaunch:
+        enforce(_RULE_RULES, self)
+        q, k, v, state, out = self.q, self.k, self.v, self.state, self.out
+        tokens, heads, K = q.shape[1:]
+        HV, V = v.shape[2:]
+        g, beta = self.g.reshape(tokens, HV), self.beta.reshape(tokens, HV)
+        if HV > 1 and (g.stride(1) != 1 or beta.stride(1) != 1):
+            fail("gate and beta heads must be contiguous")
+        pages = _row_pages(parts, tokens, state.shape[0], q.device)
+        gating = a_log = dt_bias = None
+        if self.a_log is not None:
+            a_log, dt_bias = self.a_log.data_ptr(), self.dt_bias.data_ptr()
+            self.gating = N.GatingExt(N.dtype_code(self.a_log.dtype), N.dtype_code(self.dt_bias.dtype), *self.softplus)
+            gating = ctypes.pointer(self.gating)
+        self.keep = (g, beta)  # what the pointers below name
+        strides = state.stride()
+        return N.RuleLaunch(
+            pages, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
+            state.data_ptr(), a_log, dt_bias, gating, heads, HV, K, V, q.stride(1), k.stride(1), v.stride(1),
+            g.stride(0), beta.stride(0), out.stride(1), strides[0], strides[1], strides[2], N.dtype_code(q.dtype),
+            N.dtype_code(g.dtype), N.dtype_code(beta.dtype), N.dtype_code(out.dtype), N.dtype_code(state.dtype),
+            0 if normalized else 1, K ** -0.5 if scale is None else float(scale), 0)
+
+    def prefill(self, parts, scale, normalized):
+        launch = self.launch(parts, scale, normalized)
+        lib = N.load()
+        ref = ctypes.byref(launch)
+        nbytes = lib.gdn_recoverssm_prefill_workspace(ref)
+        if nbytes < 0:
+            N.check(N.GDN_ERR_UNSUPPORTED, "prefill")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.q.device) if nbytes else None
+        N.check(lib.gdn_recoverssm_prefill(ref, N.ptr(workspace), nbytes, N.stream_handle(self.q.device)), "prefill")
+        _COUNTS["prefill"] += 1
+        return self.out
+
+    def decode(self, parts, scale, normalized):
+        launch = self.launch(parts, scale, normalized)
+        N.check(N.load().gdn_recoverssm_decode(ctypes.byref(launch), N.stream_handle(self.q.device)), "decode")
+        _COUNTS["decode"] += 1
+        return self.out
+
+
+def gdn_recoverssm_prefill(
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    checkpoint_state: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    state_indices: torch.Tensor,
+    final_indices: torch.Tensor | None = None,
+    num_computed: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    block_size: int | None = None,
+    request_indices: torch.Tensor | None = None,
+    scale: float | None = None,
+    qk_already_normalized: bool = True,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The gated delta rule over packed prompts, from each row's state page to
+    its final page (see the module's description of a row).
+
+    ``g`` (log decay) and ``beta``: [1, T, HV] or [T, HV]; ``q``, ``k``:
+    [1, T, H, K]; ``v``: [1, T, HV, V]; ``checkpoint_state``: [pages, HV, V, K].
+    Per token: c = beta (v - e^g S k); S <- e^g S + c k^T; out = scale S q
+    (``scale`` defaults to K^-0.5). With ``qk_already_normalized=False`` q and k
+    are L2-normalised in the kernel (eps 1e-6). Returns ``out`` [1, T, HV, V],
+    allocated when not given. States are computed to FP32 precision whatever the
+    activation dtype, and rounded once where a page of fewer bits is written. A
+    NaN or an infinity among a token's inputs can reach the outputs of up to 63
+    tokens before it in its own row (the chunk), besides those after it.
+
+    Working memory is taken from torch's allocator: 40 KiB per 64 tokens and
+    value head of 16-bit activations, and 16 KiB per 64 tokens and key head at
+    K = 128.
+    """
+    return _RuleCall(g, beta, q, k, v, checkpoint_state, out).prefill(
+        (query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices, block_size),
+        scale, qk_already_normalized)
+
+
+def gdn_recoverssm_prefill_gated(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    A_log: torch.Tensor,
+    dt_bias: torch.Tensor,
+    checkpoint_state: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    state_indices: torch.Tensor,
+    final_indices: torch.Tensor | None = None,
+    num_computed: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    block_size: int | None = None,
+    request_indices: torch.Tensor | None = None,
+    scale: float | None = None,
+    qk_already_normalized: bool = False,
+    softplus_beta: float = 1.0,
+    softplus_threshold: float = 20.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``gdn_recoverssm_prefill`` with the layer's gating, and by default the q/k
+    L2 norm, in the kernel, as ``gdn_recoverssm_verify_gated`` has them: per
+    token and value head g = -exp(A_log) softplus(a + dt_bias), beta =
+    sigmoid(b), in FP32, from the raw projections ``a`` and ``b``."""
+    return _RuleCall(a, b, q, k, v, checkpoint_state, out, A_log, dt_bias,
+                     (float(softplus_beta), float(softplus_threshold))).prefill(
+        (query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices, block_size),
+        scale, qk_already_normalized)
+
+
+def gdn_recoverssm_decode(
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    checkpoint_state: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    state_indices: torch.Tensor,
+    final_indices: torch.Tensor | None = None,
+    num_computed: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    block_size: int | None = None,
+    request_indices: torch.Tensor | None = None,
+    scale: float | None = None,
+    qk_already_normalized: bool = True,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``gdn_recoverssm_prefill``'s rule token by token: the arguments, pages and
+    results are the same. For requests that decode without drafts (one token a
+    row) and rows of a few tokens; each page is read and written once, whatever
+    the row's length."""
+    return _RuleCall(g, beta, q, k, v, checkpoint_state, out).decode(
+        (query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices, block_size),
+        scale, qk_already_normalized)
+
+
+def gdn_recoverssm_decode_gated(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    A_log: torch.Tensor,
+    dt_bias: torch.Tensor,
+    checkpoint_state: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    state_indices: torch.Tensor,
+    final_indices: torch.Tensor | None = None,
+    num_computed: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    block_size: int | None = None,
+    request_indices: torch.Tensor | None = None,
+    scale: float | None = None,
+    qk_already_normalized: bool = False,
+    softplus_beta: float = 1.0,
+    softplus_threshold: float = 20.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``gdn_recoverssm_decode`` with the gating and by default the q/k L2 norm in
+    the kernel (see ``gdn_recoverssm_prefill_gated``)."""
+    return _RuleCall(a, b, q, k, v, checkpoint_state, out, A_log, dt_bias,
+                     (float(softplus_beta), float(softplus_threshold))).decode(
+        (query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices, block_size),
+        scale, qk_already_normalized)
+
+
+# Taps of the convolution the kernel is built for.
+MAX_CONV_TAPS = 5
+
+_CONV_RULES = (
+    ("x must have shape [tokens, channels]", lambda x, w, b, s, o: x.ndim == 2 and x.shape[1] > 0),
+    ("conv activations, weight, bias, output and states must share one dtype (FP32, BF16 or FP16)",
+     lambda x, w, b, s, o: x.dtype in _FLOAT_TYPES
+     and all(t is None or t.dtype == x.dtype for t in (w, b, s, o))),
+    (f"weight must be contiguous [channels, taps] with 2 to {MAX_CONV_TAPS} taps",
+     lambda x, w, b, s, o: w.ndim == 2 and w.shape[0] == x.shape[1] and 2 <= w.shape[1] <= MAX_CONV_TAPS
+     and w.is_contiguous()),
+    ("bias must be contiguous [channels]",
+     lambda x, w, b, s, o: b is None or (b.ndim == 1 and b.shape[0] == x.shape[1] and b.is_contiguous())),
+    ("conv states must have shape [pages, channels, window] with a window of at least taps - 1",
+     lambda x, w, b, s, o: s.ndim == 3 and s.shape[0] > 0 and s.shape[1] == x.shape[1]
+     and s.shape[2] >= w.shape[1] - 1),
+    ("channels must be contiguous", lambda x, w, b, s, o: x.stride(1) == 1 or x.shape[1] == 1),
+    ("output shape or layout is incompatible",
+     lambda x, w, b, s, o: o.shape == x.shape and (o.stride(1) == 1 or o.shape[1] == 1)),
+    ("inputs must be on the same device",
+     lambda x, w, b, s, o: all(t is None or t.device == x.device for t in (w, b, s, o))),
+    ("the convolution runs on a HIP device", lambda x, w, b, s, o: x.device.type == "cuda"),
+)
+
+
+def gdn_recoverssm_conv(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    conv_states: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    state_indices: torch.Tensor,
+    final_indices: torch.Tensor | None = None,
+    num_computed: torch.Tensor | None = None,
+    block_table: torch.Tensor | None = None,
+    block_size: int | None = None,
+    request_indices: torch.Tensor | None = None,
+    activation: str | None = "silu",
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal depthwise convolution of packed rows (see the module's description
+    of a row), with SiLU by default.
+
+    ``x``: [T, D]; ``weight``: [D, taps]; ``bias``: [D]; ``conv_states``:
+    [pages, D, window], the layer's conv states as the commit compacts them: the
+    last taps - 1 inputs at positions 0 .. taps - 2 of the window. Tokens before
+    a row's first come from its source page; its last taps - 1 inputs go to its
+    final page (and, in align mode, those before each block boundary to that
+    boundary's page), other positions keep their values. ``activation``:
+    ``"silu"`` or None. Returns ``out`` [T, D]; it may not share memory with
+    ``x``.
+    """
+    if activation not in ("silu", None):
+        fail("activation must be 'silu' or None")
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    enforce(_CONV_RULES, x, weight, bias, conv_states, out)
+    if x.numel() and out.data_ptr() == x.data_ptr():
+        fail("the convolution's output may not share memory with its input")
+    pages = _row_pages((query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices,
+                        block_size), x.shape[0], conv_states.shape[0], x.device)
+    launch = N.ConvRows(pages, x.data_ptr(), weight.data_ptr(), N.ptr(bias), out.data_ptr(), conv_states.data_ptr(),
+                        x.shape[1], weight.shape[1], conv_states.shape[2], x.stride(0), out.stride(0),
+                        *conv_states.stride(), N.dtype_code(x.dtype), 1 if activation else 0)
+    N.check(N.load().gdn_recoverssm_conv(ctypes.byref(launch), N.stream_handle(x.device)), "conv")
+    _COUNTS["conv_rows"] += 1
+    return out
+
+
+__all__ = [
+    "MAX_CONV_TAPS",
+    "gdn_recoverssm_conv",
+    "gdn_recoverssm_decode",
+    "gdn_recoverssm_decode_gated",
+    "gdn_recoverssm_prefill",
+    "gdn_recoverssm_prefill_gated",
+]

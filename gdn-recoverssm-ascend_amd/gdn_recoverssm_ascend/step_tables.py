@@ -1,0 +1,191 @@
+"""A step's tables, built on the GPU from its rows' lengths.
+
+No counterpart in the reference, whose host framework builds them on the CPU.
+``gdn_recoverssm_step_tables`` gives a step's query offsets, token positions,
+cache slots, sequence lengths, state source and final pages, and takes the cache
+pages that the step newly needs from a ring of free ones;
+``gdn_recoverssm_release_pages`` gives the pages of ended requests back. Neither
+synchronises, so a step's metadata never visits the host.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _native as N
+from ._rules import enforce, fail
+from .kernels import _COUNTS, _INDEX_TYPES
+
+# Rows of one call (GDN_TABLES_MAX_ROWS).
+MAX_TABLE_ROWS = 4096
+
+
+@dataclass(frozen=True)
+class StepTables:
+    """What ``gdn_recoverssm_step_tables`` fills; see there. ``allocate`` makes
+    a set to be reused from step to step."""
+
+    query_start_loc: torch.Tensor  # [rows + 1] int32
+    seq_lens: torch.Tensor  # [rows] int32
+    source_indices: torch.Tensor  # [rows] int32
+    final_indices: torch.Tensor  # [rows] int32
+    new_pages: torch.Tensor  # [rows] int32
+    positions: torch.Tensor  # [num_tokens] int64
+    slot_mapping: torch.Tensor  # [num_tokens] int64
+    free_span: torch.Tensor  # [2] int64
+
+    @classmethod
+    def allocate(cls, rows: int, num_tokens: int, device) -> "StepTables":
+        # Two allocations: eight small tensors would cost more host time than the kernel takes.
+        words = torch.empty(5 * rows + 1, dtype=torch.int32, device=device)
+        longs = torch.empty(2 * num_tokens + 2, dtype=torch.int64, device=device)
+        return cls(*words.split((rows + 1, rows, rows, rows, rows)), *longs.split((num_tokens, num_tokens, 2)))
+
+
+_TABLE_RULES = (
+    ("num_computed and query_lens must be one-dimensional", lambda c: c.computed.ndim == 1 and c.lens.ndim == 1),
+    ("request_indices must have one entry per row",
+     lambda c: c.requests is None or (c.requests.ndim == 1 and c.requests.shape[0] == c.lens.shape[0])),
+    ("num_computed needs one entry per row when there are no request_indices",
+     lambda c: c.requests is not None or c.computed.shape[0] >= c.lens.shape[0]),
+    ("lengths and request indices must be int32 or int64",
+     lambda c: all(t is None or t.dtype in _INDEX_TYPES for t in (c.computed, c.lens, c.requests))),
+    (f"a call takes at most {MAX_TABLE_ROWS} rows", lambda c: c.lens.shape[0] <= MAX_TABLE_ROWS),
+    ("num_tokens must be >= 0", lambda c: c.num_tokens >= 0),
+    ("the tables run on a HIP device", lambda c: c.table.device.type == "cuda"),
+)
+
+_POOL_RULES = (
+    ("the block table must be int32 [requests, columns] with contiguous columns",
+     lambda table, free, span, block: table.ndim == 2 and table.dtype == torch.int32 and table.shape[1] > 0
+     and (table.stride(1) == 1 or table.shape[1] == 1)),
+    ("free_pages must be a contiguous int32 ring",
+     lambda table, free, span, block: free.ndim == 1 and free.dtype == torch.int32 and free.is_contiguous()
+     and free.shape[0] > 0),
+    ("free_span must be a contiguous int64 pair",
+     lambda table, free, span, block: tuple(span.shape) == (2,) and span.dtype == torch.int64 and span.stride(0) == 1),
+    ("block_size must be positive", lambda table, free, span, block: block > 0),
+    ("inputs must be on the same device",
+     lambda table, free, span, block: table.device == free.device == span.device),
+)
+
+
+class _TableCall:
+    def __init__(self, table, computed, lens, requests, num_tokens):
+        self.table, self.computed, self.lens, self.requests = table, computed, lens, requests
+        self.num_tokens = int(num_tokens)
+
+
+def gdn_recoverssm_step_tables(
+    block_table: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_span: torch.Tensor,
+    *,
+    num_computed: torch.Tensor,
+    query_lens: torch.Tensor,
+    block_size: int,
+    num_tokens: int,
+    request_indices: torch.Tensor | None = None,
+    out: StepTables | None = None,
+) -> StepTables:
+    """Build a step's tables from its rows' lengths.
+
+    Row r describes request ``request_indices[r]`` (default r) with C =
+    ``num_computed[request]`` cached tokens and n = ``query_lens[r]`` new ones;
+    columns 0 .. ceil(C / block_size) - 1 of its ``block_table`` row hold its
+    pages. Columns up to ceil((C + n) / block_size) - 1 take new ones from the
+    ring ``free_pages``, whose places ``free_span`` = [head, tail) (counters that
+    only grow, taken modulo the ring's length) hold the free pages. Rows take
+    pages in order; a row that no longer fits, or whose request or columns lie
+    outside the table, is refused (``new_pages`` -1, slots -1, final page 0) and
+    takes nothing.
+
+    Returns ``StepTables``: ``query_start_loc``; ``positions`` and
+    ``slot_mapping`` (page * block_size + position % block_size) of
+    ``num_tokens`` tokens (the step's, or more: -1 past the last); ``seq_lens`` =
+    C + n; ``source_indices``, the page of the block that token C - 1 lies in (0
+    for a new request); ``final_indices``, that of token C + n - 1; ``new_pages``
+    per row; and the ring's new ``free_span``, to be passed to the next step
+    (a buffer of its own: ``out.free_span`` must not be ``free_span``).
+    ``block_table`` is filled in place.
+    """
+    c = _TableCall(block_table, num_computed, query_lens, request_indices, num_tokens)
+    enforce(_TABLE_RULES, c)
+    enforce(_POOL_RULES, block_table, free_pages, free_span, block_size)
+    rows, device = query_lens.shape[0], block_table.device
+    if any(t is not None and t.device != device for t in (num_computed, query_lens, request_indices)):
+        fail("inputs must be on the same device")
+    if out is None:
+        out = StepTables.allocate(rows, c.num_tokens, device)
+    else:
+        _check_out(out, rows, c.num_tokens, device, free_span)
+    requests = request_indices
+    launch = N.StepTablesLaunch(
+        num_computed.data_ptr(), query_lens.data_ptr(), N.ptr(requests), block_table.data_ptr(),
+        free_pages.data_ptr(), free_span.data_ptr(), out.free_span.data_ptr(), out.query_start_loc.data_ptr(),
+        out.seq_lens.data_ptr(), out.source_indices.data_ptr(), out.final_indices.data_ptr(),
+        out.new_pages.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), rows, c.num_tokens,
+        num_computed.shape[0], num_computed.stride(0), query_lens.stride(0),
+        0 if requests is None else requests.stride(0), block_table.shape[0], block_table.shape[1],
+        block_table.stride(0), free_pages.shape[0], block_size, N.dtype_code(num_computed.dtype),
+        N.dtype_code(query_lens.dtype), N.DT_I32 if requests is None else N.dtype_code(requests.dtype), 0)
+    N.check(N.load().gdn_recoverssm_step_tables(ctypes.byref(launch), N.stream_handle(device)), "step_tables")
+    _COUNTS["step_tables"] += 1
+    return out
+
+
+def _check_out(out: StepTables, rows: int, num_tokens: int, device, free_span) -> None:
+    shapes = (("query_start_loc", rows + 1, torch.int32), ("seq_lens", rows, torch.int32),
+              ("source_indices", rows, torch.int32), ("final_indices", rows, torch.int32),
+              ("new_pages", rows, torch.int32), ("positions", num_tokens, torch.int64),
+              ("slot_mapping", num_tokens, torch.int64), ("free_span", 2, torch.int64))
+    for name, length, dtype in shapes:
+        t = getattr(out, name)
+        if t.shape != (length,) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+            fail(f"out.{name} must be contiguous {dtype} [{length}] on the tables' device")
+    if out.free_span.data_ptr() == free_span.data_ptr():
+        fail("out.free_span must not be free_span")
+
+
+def gdn_recoverssm_release_pages(
+    block_table: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_span: torch.Tensor,
+    *,
+    requests: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_size: int,
+) -> torch.Tensor:
+    """Give the pages of ended requests back to the ring of free pages.
+
+    For each entry of ``requests`` in order (none twice): the non-null entries of
+    columns 0 .. ceil(``seq_lens[i]`` / block_size) - 1 of its ``block_table`` row
+    are put behind the ring's tail and become 0. Returns the ring's new span.
+    The ring must have room for every page of the pool that can be free at once
+    (a ring as long as the pool has).
+    """
+    enforce(_POOL_RULES, block_table, free_pages, free_span, block_size)
+    enforce((
+        ("requests and seq_lens must be one-dimensional, one entry per ended request",
+         lambda: requests.ndim == 1 and seq_lens.ndim == 1 and requests.shape == seq_lens.shape),
+        ("requests and seq_lens must be int32 or int64",
+         lambda: requests.dtype in _INDEX_TYPES and seq_lens.dtype in _INDEX_TYPES),
+        ("requests must be contiguous", lambda: requests.is_contiguous()),
+        ("inputs must be on the same device",
+         lambda: requests.device == seq_lens.device == block_table.device),
+        ("the tables run on a HIP device", lambda: block_table.device.type == "cuda"),
+    ))
+    span = torch.empty_like(free_span)
+    N.check(N.load().gdn_recoverssm_release_pages(
+        requests.data_ptr(), N.dtype_code(requests.dtype), requests.shape[0], seq_lens.data_ptr(),
+        N.dtype_code(seq_lens.dtype), seq_lens.stride(0), block_table.data_ptr(), block_table.shape[0],
+        block_table.shape[1], block_table.stride(0), block_size, free_pages.data_ptr(), free_pages.shape[0],
+        free_span.data_ptr(), span.data_ptr(), N.stream_handle(block_table.device)), "release_pages")
+    _COUNTS["release_pages"] += 1
+    return span
+
+
+__all__ = ["MAX_TABLE_ROWS", "StepTables", "gdn_recoverssm_release_pages", "gdn_recoverssm_step_tables"]

@@ -28,6 +28,10 @@
  *   gdn_recoverssm_set_state_cache_retain -> no counterpart: a cache hint for the verify launches
  *   gdn_recoverssm_settle        -> no counterpart: which pending rows of a deferred commit a
  *                                   settle folds (the next verifies do not apply them)
+ *   gdn_recoverssm_prefill, gdn_recoverssm_prefill_workspace, gdn_recoverssm_decode,
+ *   gdn_recoverssm_conv, gdn_recoverssm_step_tables, gdn_recoverssm_release_pages
+ *                                -> no counterpart: the prompt and the plain decode of the layer
+ *                                   whose speculative windows the entries above serve
  */
 #ifndef GDN_RECOVERSSM_HIP_H
 #define GDN_RECOVERSSM_HIP_H
@@ -418,6 +422,153 @@ typedef struct gdn_settle_next {
 int gdn_recoverssm_settle(int32_t *lengths, const int32_t *finals, int64_t num_groups, int64_t capacity,
                           int64_t num_rows, const int32_t *rows, int64_t rows_len, const gdn_settle_next *next,
                           int32_t *out_lengths, int32_t *row_list, int32_t *row_count, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * The prompt and the plain decode of the layer (no counterpart in the
+ * reference, which leaves both to its host framework).
+ * ------------------------------------------------------------------------ */
+
+/* Where each row's tokens lie, which page its state starts from and which
+ * page it ends in. DEVICE arrays. Row b has tokens query_start_loc[b] ..
+ * query_start_loc[b + 1] - 1 and describes request req = request_indices[b]
+ * (b when NULL), whose first C = num_computed[req] tokens came before. Its
+ * state starts at zero when num_computed is given and C = 0 (no page is read
+ * then), else from page state_indices[b]. It ends in page
+ *   block_table[req][min((C + n - 1) / block_size, table_width - 1)]  (block_table given), else
+ *   final_indices[b] (when not NULL), else state_indices[b],
+ * and with a block table the state at every block boundary that lies inside
+ * the row, p with C < p < C + n and p % block_size = 0, also goes to page
+ * block_table[req][p / block_size - 1] where that is a valid page other than
+ * the final one. A page is valid in 1 .. blocks - 1 (page 0 is the null page).
+ * A row with an invalid final page, an invalid source page that it would have
+ * to read, a request index outside computed_len / table_rows or C < 0 gives
+ * zero outputs and stores nothing; a row without tokens does nothing. Pages of
+ * different rows must not coincide; a row's own may. Strides in elements. */
+typedef struct gdn_row_pages {
+  const void *query_start_loc;  /* [rows + 1] */
+  const void *state_indices;    /* [rows] */
+  const void *final_indices;    /* [rows] or NULL; NULL with a block table */
+  const void *num_computed;     /* [computed_len] or NULL */
+  const void *block_table;      /* [table_rows, table_width] or NULL; needs num_computed and block_size */
+  const void *request_indices;  /* [rows] or NULL */
+  int64_t rows, tokens, blocks;
+  int64_t qsl_stride, si_stride, final_stride, computed_stride, map_stride;
+  int64_t computed_len;
+  int64_t table_row_stride, table_col_stride, table_rows, table_width, block_size;
+  int32_t qsl_dtype, si_dtype, final_dtype, computed_dtype, map_dtype, table_dtype; /* I32 / I64 */
+} gdn_row_pages;
+
+/* The gated delta rule over whole rows. Per token and value head, in FP32:
+ *   c = beta (v - e^g S k),  S <- e^g S + c k^T,  out = scale S q.
+ * q, k: [1, T, H, K]; v, out: [1, T, HV, V]; g, beta: [T, HV] (heads
+ * contiguous, token strides free); state: [blocks, HV, V, K] (K contiguous,
+ * rows 16-byte aligned). qk_l2norm: q and k are L2-normalised first (eps
+ * 1e-6). gating: g and beta hold the raw projections a and b, see
+ * gdn_gating_ext. */
+typedef struct gdn_rule_launch {
+  gdn_row_pages pages;
+  const void *q, *k, *v, *g, *beta;
+  void *out, *state;
+  const void *a_log, *dt_bias;        /* [HV], with gating */
+  const gdn_gating_ext *gating;       /* HOST pointer, or NULL */
+  int64_t heads, value_heads, key_dim, value_dim;
+  int64_t q_stride, k_stride, v_stride, g_stride, beta_stride, out_stride; /* per token */
+  int64_t state_block_stride, state_head_stride, state_v_stride;
+  int32_t act_dtype;                  /* q, k, v: F32 / BF16 / F16 */
+  int32_t g_dtype, beta_dtype, out_dtype; /* the activation dtype or F32 */
+  int32_t state_dtype;                /* F32 / BF16 / F16 */
+  int32_t qk_l2norm;
+  float scale;
+  int32_t reserved;
+} gdn_rule_launch;
+
+/* Recurrent form: every row's tokens one after the other, its state in
+ * registers between them. For rows of one or a few tokens. */
+int gdn_recoverssm_decode(const gdn_rule_launch *launch, void *stream);
+
+/* Chunked form, on the matrix cores, for prompts: 64 tokens at a time (a chunk
+ * also ends at a block boundary). Results are those of the recurrent form up
+ * to FP32 rounding, except that a NaN or an infinity among a token's inputs
+ * also reaches the tokens before it in its chunk. `workspace` is DEVICE memory
+ * of at least gdn_recoverssm_prefill_workspace(launch) bytes, 16-byte aligned,
+ * of which nothing outlives the call. The size depends on the counts, dims
+ * and dtypes of `launch` alone; it is negative for a launch that
+ * gdn_recoverssm_prefill rejects. */
+int64_t gdn_recoverssm_prefill_workspace(const gdn_rule_launch *launch);
+int gdn_recoverssm_prefill(const gdn_rule_launch *launch, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Causal depthwise convolution of packed rows with its state pages:
+ *   out[t][d] = act(bias[d] + sum_j weight[d][j] x[t - taps + 1 + j][d]),
+ * where positions before the row's first token come from its source page
+ * (zero where its state starts at zero): conv_states [blocks, D, window] holds
+ * the last taps - 1 inputs at token positions 0 .. taps - 2 (window >= taps -
+ * 1), the layout of gdn_recoverssm_conv_compact. The row's last taps - 1
+ * inputs go to its final page (and those before a block boundary to that
+ * boundary's page) the same way; other positions of a page keep their values.
+ * x, out: [T, D] with D contiguous; weight: [D, taps] contiguous, 2 <= taps <=
+ * 5; bias: [D] or NULL; x, weight, bias, out and conv_states share one dtype.
+ * FP32 arithmetic. silu: act(y) = y / (1 + e^-y), else act(y) = y. */
+typedef struct gdn_conv_rows {
+  gdn_row_pages pages;
+  const void *x, *weight, *bias;
+  void *out, *conv_states;
+  int64_t dim, taps, window;
+  int64_t x_stride, out_stride;
+  int64_t state_block_stride, state_dim_stride, state_token_stride;
+  int32_t dtype;
+  int32_t silu;
+} gdn_conv_rows;
+int gdn_recoverssm_conv(const gdn_conv_rows *launch, void *stream);
+
+/* A step's tables from its rows' lengths, on the device. Row r describes
+ * request req = request_indices[r] (r when NULL), with C = num_computed[req]
+ * tokens cached and n = query_lens[r] new ones (each < 0 counts as 0). Block
+ * table entries [req][0 .. ceil(C / block_size)) are its pages; columns
+ * ceil(C / bs) .. ceil((C + n) / bs) - 1 take new pages from a ring of free
+ * ones: free_pages [free_len] holds the free pages at places head .. tail - 1
+ * (mod free_len), free_span = {head, tail} ever growing counters. Rows take
+ * pages in row order; a row whose pages no longer fit, whose request lies
+ * outside the table or which would need more than table_width columns is
+ * refused: its new_pages is -1, its slots -1, its final page 0, and it takes
+ * nothing (as do the rows after one that no longer fitted, where they need
+ * pages). Outputs: query_start_loc [rows + 1]; per token t < num_tokens of
+ * row r, positions = C + i and slot_mapping = page * block_size + position %
+ * block_size (both -1 past the last token); per row seq_lens = C + n,
+ * source_indices = the page of block (C - 1) / bs (0 when C = 0),
+ * final_indices = the page of block (C + n - 1) / bs (0 when C + n = 0),
+ * new_pages = pages taken (num_tokens must be at least the step's tokens: the
+ * token that opens a new page also writes its table entry); free_span_out = {head + taken, tail}. free_span_out
+ * must not be free_span. At most GDN_TABLES_MAX_ROWS rows. */
+#define GDN_TABLES_MAX_ROWS 4096
+typedef struct gdn_step_tables {
+  const void *num_computed;    /* [computed_len] */
+  const void *query_lens;      /* [rows] */
+  const void *request_indices; /* [rows] or NULL */
+  int32_t *block_table;        /* [table_rows, table_width] */
+  const int32_t *free_pages;
+  const int64_t *free_span;
+  int64_t *free_span_out;
+  int32_t *query_start_loc, *seq_lens, *source_indices, *final_indices, *new_pages;
+  int64_t *positions, *slot_mapping;
+  int64_t rows, num_tokens, computed_len, computed_stride, lens_stride, map_stride;
+  int64_t table_rows, table_width, table_row_stride; /* columns contiguous */
+  int64_t free_len, block_size;
+  int32_t computed_dtype, lens_dtype, map_dtype; /* I32 / I64 */
+  int32_t reserved;
+} gdn_step_tables;
+int gdn_recoverssm_step_tables(const gdn_step_tables *launch, void *stream);
+
+/* Gives the pages of requests that ended back to the ring: for each listed
+ * request, in order, table entries [req][0 .. ceil(seq_len / block_size)) that
+ * are not 0 go to places tail, tail + 1, ... and become 0. free_span_out =
+ * {head, tail + given}; it must not be free_span. A request outside the table
+ * gives nothing; no request may be listed twice. Pages that would pass
+ * free_len free ones are dropped (a ring as long as the pool never is). */
+int gdn_recoverssm_release_pages(const void *requests, int32_t requests_dtype, int64_t num_requests,
+                                 const void *seq_lens, int32_t lens_dtype, int64_t lens_stride,
+                                 int32_t *block_table, int64_t table_rows, int64_t table_width,
+                                 int64_t table_row_stride, int64_t block_size, int32_t *free_pages,
+                                 int64_t free_len, const int64_t *free_span, int64_t *free_span_out, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,149 @@
+"""The causal convolution of packed rows on the GPU against its definition in 64
+bits. States are copies of inputs: bit-exact. Outputs are FP32 sums rounded once:
+norm-wise 2^-8 BF16, 2^-11 F16, 1e-6 FP32."""
+
+import pytest
+import torch
+
+import gdn_recoverssm_ascend as G
+import prompt_oracle as P
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+TOL = {torch.float32: 1e-6, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+NAMES = dict(final="final_indices", computed="num_computed", table="block_table", requests="request_indices")
+
+
+def problem(lengths, D, taps, dtype, window=None, seed=0, bias=True, pages=None):
+    gen = torch.Generator().manual_seed(seed)
+    randn = lambda *s: torch.randn(*s, generator=gen).to(DT[dtype])  # noqa: E731
+    B = len(lengths)
+    window = taps - 1 if window is None else window
+    place = 1 + torch.randperm(2 * B, generator=gen)
+    return dict(x=randn(sum(lengths), D), weight=randn(D, taps), bias=randn(D) if bias else None,
+                states=randn(pages or 2 * B + 2, D, window), source=place[:B].int(), final=place[B:].int(),
+                qsl=torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32))
+
+
+def check(p, dev, *, rows=None, silu=True, states=None, **call):
+    rows = rows or {}
+    want, after = P.conv(p["x"], p["weight"], p["bias"], p["states"], p["qsl"], p["source"], silu=silu, **rows)
+    kw = {NAMES[n]: t.to(dev) for n, t in rows.items() if n in NAMES}
+    if "block" in rows:
+        kw["block_size"] = rows["block"]
+    states = p["states"].to(dev) if states is None else states
+    out = G.gdn_recoverssm_conv(call.pop("x", p["x"].to(dev)), p["weight"].to(dev),
+                                None if p["bias"] is None else p["bias"].to(dev), conv_states=states,
+                                query_start_loc=p["qsl"].to(dev), state_indices=p["source"].to(dev),
+                                activation="silu" if silu else None, **kw, **call)
+    torch.cuda.synchronize()
+    err = float((out.cpu().double() - want).norm() / want.norm().clamp(min=1e-30)) if want.numel() else 0.0
+    assert err <= TOL[out.dtype], f"out: {err:.3g}"
+    zero = (want == 0).all(1)
+    assert not out.cpu()[zero].any()
+    assert torch.equal(states.cpu(), after)
+    return out
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("taps", [2, 3, 4, 5])
+@pytest.mark.parametrize("lengths", [[1], [1, 1, 1, 1, 1], [2, 3, 1, 0, 4], [40, 1, 0, 65, 2], [200], [31, 32, 33]],
+                         ids=lambda v: "-".join(map(str, v)))
+def test_rows(lengths, taps, dtype, gpu_device):
+    p = problem(lengths, 300, taps, dtype, seed=taps, bias=taps % 2 == 0)
+    check(p, gpu_device, rows=dict(final=p["final"]), silu=taps != 3)
+
+
+@pytest.mark.parametrize("D", [1, 2, 7, 8, 9, 511, 512, 513, 2048, 2051])
+@pytest.mark.parametrize("lengths", [[1, 2, 1], [50, 30]], ids=["short", "long"])
+def test_channels(lengths, D, gpu_device):
+    p = problem(lengths, D, 4, "bf16", window=6, seed=D)
+    check(p, gpu_device, rows=dict(final=p["final"]))
+
+
+@pytest.mark.parametrize("window", [3, 4, 6, 7, 11])
+@pytest.mark.parametrize("lengths", [[1, 2, 3, 4], [70, 1]], ids=["short", "long"])
+def test_in_place_windows(lengths, window, gpu_device):
+    """Source and final page the same, rows shorter than the history; the
+    window behind the history keeps its bits."""
+    p = problem(lengths, 130, 4, "bf16", window=window, seed=window)
+    check(p, gpu_device)
+
+
+@pytest.mark.parametrize("lengths", [[5, 1, 2, 70, 3, 4, 1], [1, 1, 1, 1, 1, 1, 1]], ids=["mixed", "single"])
+def test_refused_rows_and_zero_starts(lengths, gpu_device):
+    p = problem(lengths, 64, 4, "bf16", seed=4)
+    p["states"][int(p["source"][1])] = float("nan")
+    p["source"][0] = 0
+    p["source"][2] = p["states"].shape[0]
+    p["source"][3] = -1
+    p["final"][4] = 0
+    p["final"][5] = 1000
+    rows = dict(final=p["final"], computed=torch.tensor([5, 0, 7, 0, 0, 2, -3]))
+    # The NaN page is read by nobody and changes nowhere: compared as bits.
+    want, after = P.conv(p["x"], p["weight"], p["bias"], p["states"], p["qsl"], p["source"], **rows)
+    states = p["states"].to(gpu_device)
+    out = G.gdn_recoverssm_conv(p["x"].to(gpu_device), p["weight"].to(gpu_device), p["bias"].to(gpu_device),
+                                conv_states=states, query_start_loc=p["qsl"].to(gpu_device),
+                                state_indices=p["source"].to(gpu_device), final_indices=p["final"].to(gpu_device),
+                                num_computed=rows["computed"].to(gpu_device)).cpu()
+    assert not out.isnan().any()
+    assert float((out.double() - want).norm() / want.norm()) <= TOL[out.dtype]
+    assert torch.equal(states.cpu().view(torch.int16), after.view(torch.int16))
+
+
+@pytest.mark.parametrize("block", [1, 2, 16, 33, 64, 128])
+def test_block_table(block, gpu_device):
+    """Boundary histories go to the boundaries' pages; a boundary's page can be
+    the source page."""
+    lengths = [1, 63, 2, 130, 0, 97]
+    C = torch.tensor([0, 3, 64, 31, 9, 2 * block])
+    table = torch.zeros(len(lengths), max((int(c) + n) // block + 1 for c, n in zip(C, lengths)), dtype=torch.int64)
+    pages = 1
+    source = []
+    for r, (c, n) in enumerate(zip(C.tolist(), lengths)):
+        for col in range(max(c - 1, 0) // block, (c + max(n, 1) - 1) // block + 1):
+            table[r, col] = pages
+            pages += 1
+        source.append(int(table[r, max(c - 1, 0) // block]))
+    p = problem(lengths, 70, 4, "f16", window=6, seed=block, pages=pages)
+    p["source"] = torch.tensor(source)
+    check(p, gpu_device, rows=dict(computed=C, table=table, block=block))
+
+
+def test_strides(gpu_device):
+    """Tokens of a wider tensor, transposed states, output with gaps."""
+    dev = gpu_device
+    for lengths in ([40, 70, 1], [1, 1, 2]):
+        p = problem(lengths, 96, 4, "bf16", window=5, seed=7)
+        T = sum(lengths)
+        x = torch.zeros(T, 105, dtype=torch.bfloat16, device=dev)
+        x[:, 3:99] = p["x"].to(dev)
+        states = torch.zeros(p["states"].shape[0], 5, 100, dtype=torch.bfloat16, device=dev).transpose(1, 2)[:, :96]
+        states.copy_(p["states"].to(dev))
+        out = torch.full((T, 101), 5.0, dtype=torch.bfloat16, device=dev)
+        check(p, dev, rows=dict(final=p["final"]), x=x[:, 3:99], states=states, out=out[:, :96])
+        assert (out[:, 96:] == 5.0).all()
+
+
+def test_graph_replays(gpu_device):
+    dev = gpu_device
+    p = problem([60, 1, 9], 256, 4, "bf16", seed=8)
+    t = {n: p[n].to(dev) for n in ("x", "weight", "bias", "qsl", "source", "final")}
+    states = p["states"].to(dev)
+
+    def call():
+        return G.gdn_recoverssm_conv(t["x"], t["weight"], t["bias"], conv_states=states, query_start_loc=t["qsl"],
+                                     state_indices=t["source"], final_indices=t["final"])
+
+    want, after = call(), states.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for _ in range(3):
+        states.copy_(p["states"])
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(states, after)
