@@ -5,9 +5,8 @@
 namespace gdn {
 
 struct PrefillPlan {
-  int kp, pl, opl, nv;
-  bool pack;
-  int64_t bytes, scan_grid;
+  int kp, pl, opl, nw;
+  int64_t key_bytes, bytes, scan_grid;
 };
 
 static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &p, int *status) {
@@ -24,6 +23,18 @@ static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &
   a.K = int32_t(K), a.V = int32_t(V), a.H = int32_t(H), a.HV = int32_t(HV), a.ratio = int32_t(HV / H);
   a.g_dt = l->g_dtype, a.beta_dt = l->beta_dtype, a.state_dt = l->state_dtype;
   a.out_f32 = l->out_dtype == GDN_DT_F32, a.l2norm = l->qk_l2norm, a.scale = l->scale;
+  // One token's stride says nothing; the kernels then step by its own width.
+  if (rp.tokens == 1) a.v_ts = a.out_ts = HV * V;
+  // Rows of V and of the output are told apart by their offsets, which are 32
+  // bits from a chunk's first token.
+  for (int64_t ts : {a.v_ts, a.out_ts}) {
+    if (ts < V || ts > kScanReach - V) {
+      set_error("prefill: token strides of v and out must be at least the value dim and span under 1 GiB per %d tokens",
+                kChunk);
+      *status = GDN_ERR_UNSUPPORTED;
+      return false;
+    }
+  }
   // A row of n tokens spans at most n * per_block / block + 3 chunks wherever it
   // starts, and ceil(n / 64) where chunks start with the row.
   a.align = rp.block_table != nullptr;
@@ -32,34 +43,16 @@ static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &
   a.slack = a.align ? 3 : 1;
   const int64_t slots = rp.tokens * a.per_block / a.block + a.slack * rp.rows;
   p.kp = K <= 64 ? 64 : K <= 128 ? 128 : 256;
-  // BF16 keys are read in place as operands where every 8 of them start on a
-  // dword; else, and for wider types, prepare packs them as planes.
-  const bool rows_of_dwords = K % 8 == 0 && l->q_stride % 2 == 0 && l->k_stride % 2 == 0 &&
-                              (reinterpret_cast<uintptr_t>(l->q) | reinterpret_cast<uintptr_t>(l->k)) % 4 == 0;
-  const bool exact_out = a.out_f32 || l->act_dtype == GDN_DT_F32;
-  p.pack = exact_out || l->act_dtype != GDN_DT_BF16 || !rows_of_dwords;
-  p.pl = exact_out ? 3 : p.pack ? 2 : 1;
-  p.opl = exact_out ? 3 : 2;
-  int64_t at = 0;
-  const auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += bytes;
-    return here;
-  };
-  const int64_t key_planes = slots * H * 4 * (p.kp / 32) * p.pl * kFrag;
-  a.kt_at = take(key_planes);
-  a.k_at = take(p.pack ? key_planes : 0);
-  a.q_at = take(p.pack ? key_planes : 0);
-  a.t_at = take(slots * HV * 8 * kPlanesT * kFrag);
-  a.p_at = take(slots * HV * 8 * p.opl * kFrag);
-  a.s_at = take(slots * HV * kScalars * 4);
-  p.bytes = at;
-  const int64_t wide = rp.rows * HV * ((V + 31) / 32);
-  p.nv = wide >= 512 ? 2 : 1;
-  a.slices = int32_t((V + 16 * p.nv - 1) / (16 * p.nv));
+  p.pl = l->act_dtype == GDN_DT_F32 ? 2 : 1;
+  p.opl = l->act_dtype == GDN_DT_BF16 && !a.out_f32 ? 1 : 2;
+  p.key_bytes = slots * H * (12 * (p.kp / 32) * p.pl) * kUnit;
+  p.bytes = p.key_bytes + slots * HV * (14 + 6 * p.opl) * kUnit;
+  const int64_t tiles = rp.rows * HV * ((V + 15) / 16);
+  p.nw = !scan_staged(p.pl, p.opl, p.kp) ? 4 : tiles <= 256 ? 1 : tiles <= 512 ? 2 : tiles <= 1024 ? 4 : 8;
+  a.slices = int32_t((V + 16 * p.nw - 1) / (16 * p.nw));
   a.members = a.ratio * a.slices;
   p.scan_grid = (rp.rows * H + 7) / 8 * 8 * a.members;
-  if (slots * H > 0x7fffffffLL || p.scan_grid > 0x7fffffffLL || rp.rows * H > 0x7fffffffLL) {
+  if (slots * HV > 0x7fffffffLL || p.scan_grid > 0x7fffffffLL || rp.rows * H > 0x7fffffffLL) {
     set_error("prefill: grid too large");
     *status = GDN_ERR_UNSUPPORTED;
     return false;
@@ -95,14 +88,14 @@ extern "C" int gdn_recoverssm_prefill(const gdn_rule_launch *l, void *workspace,
     return GDN_ERR_INVALID;
   }
   a.ws = static_cast<char *>(workspace);
+  a.ws_value = a.ws + p.key_bytes;
   auto s = static_cast<hipStream_t>(stream);
   const unsigned grid = unsigned(p.scan_grid);
-  if (p.pl == 1) launch_prefill<bf16, 1, 2, false>(p.kp, p.nv, grid, s, a);
-  else if (l->act_dtype == GDN_DT_F32) launch_prefill<float, 3, 3, true>(p.kp, p.nv, grid, s, a);
-  else if (l->act_dtype == GDN_DT_F16 && p.pl == 2) launch_prefill<f16, 2, 2, true>(p.kp, p.nv, grid, s, a);
-  else if (l->act_dtype == GDN_DT_F16) launch_prefill<f16, 3, 3, true>(p.kp, p.nv, grid, s, a);
-  else if (p.pl == 2) launch_prefill<bf16, 2, 2, true>(p.kp, p.nv, grid, s, a);
-  else launch_prefill<bf16, 3, 3, true>(p.kp, p.nv, grid, s, a);
+  if (l->act_dtype == GDN_DT_F32) launch_prefill<float, float>(p.kp, p.nw, grid, s, a);
+  else if (l->act_dtype == GDN_DT_F16 && a.out_f32) launch_prefill<f16, float>(p.kp, p.nw, grid, s, a);
+  else if (l->act_dtype == GDN_DT_F16) launch_prefill<f16, f16>(p.kp, p.nw, grid, s, a);
+  else if (a.out_f32) launch_prefill<bf16, float>(p.kp, p.nw, grid, s, a);
+  else launch_prefill<bf16, bf16>(p.kp, p.nw, grid, s, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) {
     set_error("prefill: launch failed: %s", hipGetErrorString(err));

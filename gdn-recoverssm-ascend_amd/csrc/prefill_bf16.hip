@@ -1,7 +1,6 @@
-// The chunked rule's kernels: activation type, planes of K and Q, planes of the
-// output's products, K and Q packed by prepare.
+// The chunked rule's kernels: types of the activations and of the output.
 #include "prefill_kernel.cuh"
 
 namespace gdn {
-GDN_PREFILL(bf16, 1, 2, false)
+GDN_PREFILL(bf16, bf16)
 }

@@ -10,34 +10,40 @@
 //   S1  = e^{G_end} S0 + (diag(e^{G_end - G}) c)^T K
 // T and P depend on no state, so a first kernel (prepare) makes them for all
 // chunks at once; a second (scan) walks each (row, value head) through its
-// chunks with a slice of the state's V rows in registers.
+// chunks with the state in registers.
 //
-// Precision: states and corrections are FP32, and their products run on the
-// BF16 matrix cores with each FP32 operand as the sum of three BF16 planes of 8
-// bits (cut, not rounded: the sum of the three is the FP32 value). A product
-// takes the pairs of planes whose places add up to at most 2, which drops terms
-// under 2^-24 of it. BF16 keys are one plane, F16 two, FP32 three. The output's
-// own products take OPL planes, two (2^-16) where it is rounded to 16 bits.
-// The FP32 matrix instruction would take 16 times a BF16 one's time, 3 to 6
-// times what the planes take.
+// Precision: states and corrections are FP32, and their products run on the F16
+// matrix cores with an FP32 operand as the sum of two F16 planes of 11 bits (its
+// rounding to F16, and that of what the rounding left: 2^-23 of a value). F16
+// has no FP32's range, so every operand is scaled by powers of two, which cost
+// no bits: rows of K and Q by their largest element, T by nothing (|T| <= 2
+// where the rule is stable), and all that is linear in a column of V (S0, v, c,
+// out) by one factor a column that the scan follows from chunk to chunk. A
+// product of two split operands drops the two low planes' product, 2^-24 of it.
+// Outputs rounded to BF16 take one plane of S0, P and c (2^-12); F16 and FP32
+// ones two. Three BF16 planes need no scaling and were tried first: 1.5 times
+// the products and planes, and twice the instructions that make them. The FP32
+// matrix instruction takes 16 times an F16 one's time.
 //
 // With the L2 norm fused in, 1 / |k| and 1 / |q| go into the scalars beside T,
 // P and the decays, and K and Q stay as they are.
 #pragma once
+
+#include <type_traits>
 
 #include "rows.cuh"
 
 namespace gdn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kChunk = 64;
-constexpr int kPrefillThreads = 256;
-constexpr int kPlanesT = 3;
-constexpr int kFrag = 1024;            // bytes of one 16 x 32 operand plane
+constexpr int kUnit = 1024;            // bytes of one 16 x 32 operand plane
 constexpr float kMinLogDecay = -200.f; // e^-200 is 0 in FP32: cumulative sums stay finite
 
 struct PrefillArgs {
@@ -54,20 +60,38 @@ struct PrefillArgs {
   // `block` tokens, per_block chunks each; row b's chunks start at slot
   // qsl[b] * per_block / block + slack * b, which leaves every row enough.
   int32_t align, block, per_block, slack, slots;
-  // Workspace: per (slot, key head) K^T (and packed K, Q), per (slot, value
-  // head) T, P and the scalars.
-  char *ws;
-  int64_t kt_at, k_at, q_at, t_at, p_at, s_at;
-  int32_t slices, members;  // scan: V slices of a state, workgroups of a key head's group
+  char *ws;        // per (slot, key head): K, Q, K^T
+  char *ws_value;  // per (slot, value head): T, P, scalars
+  int32_t slices, members;  // scan: workgroups of a state, of a key head's group
 };
 
-// Scalars of a (slot, value head): floats [4][64].
-constexpr int kScalars = 4 * kChunk;
-enum { kScIn = 0, kScQ = kChunk, kScOut = 2 * kChunk, kScEnd = 3 * kChunk };
+// Operand planes in the workspace, in units of 1 KB (64 lanes x 8 F16):
+//   key head:   K (token tile, 32 columns, plane), Q alike, K^T (16 columns,
+//               32 tokens, plane);
+//   value head: T (the six 16 x 32 blocks that are not zero, 2 planes), P
+//               (alike, OPL planes), scalars (2 units).
+// The 32 columns k of an operand are in the order in which an accumulator's
+// rows lie in the lanes: lane quarter lq has k = 4 lq .. 4 lq + 3 and 16 + 4 lq
+// .. 16 + 4 lq + 3. So two accumulator tiles of one wave, as they are, make the
+// other operand of the next product, and the scan moves no value from lane to
+// lane.
+template <typename A>
+constexpr int key_planes() { return sizeof(A) == 4 ? 2 : 1; }  // of K and Q
+template <typename Out>
+constexpr int out_planes() { return std::is_same<Out, bf16>::value ? 1 : 2; }  // of S0, P and c in the output
+template <typename A, typename Out, int KP>
+struct Units {
+  static constexpr int PL = key_planes<A>(), OPL = out_planes<Out>(), KS = KP / 32;
+  static constexpr int Q = 4 * KS * PL, KT = 8 * KS * PL, KEY = 12 * KS * PL;
+  static constexpr int P = 12, SC = 12 + 6 * OPL, VALUE = SC + 2;
+};
+// Block (token tile, 32 columns) of T and P.
+__host__ __device__ constexpr int lower_block(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
+// Scalars of a (slot, value head): arrays of 64 floats.
+enum { kScIn = 0, kScQ = 1, kScOut = 2, kScMul = 3, kScEnd = 4 };
 
-__device__ __forceinline__ int64_t first_slot(const PrefillArgs &a, int b) {
-  const int64_t at = load_index(a.pages.query_start_loc, b * a.pages.qsl_stride, a.pages.qsl_dtype);
-  return int64_t(clamp_token(at, a.pages.tokens)) * a.per_block / a.block + int64_t(a.slack) * b;
+__device__ __forceinline__ int64_t slot_of(const PrefillArgs &a, int b, int first_token) {
+  return int64_t(first_token) * a.per_block / a.block + int64_t(a.slack) * b;
 }
 
 // Orders LDS across the workgroup without draining global loads in flight.
@@ -78,105 +102,135 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// x as PL planes of its leading 8 bits and what they leave, packed pairwise.
-template <int PL, int N>
-__device__ __forceinline__ void split(const float (&x)[N], uint32_t (&planes)[PL][N / 2]) {
+// Two values as PL planes.
+template <int PL>
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&planes)[PL]) {
+  const f16x2 hi = __builtin_convertvector(f32x2{a, b}, f16x2);
+  planes[0] = __builtin_bit_cast(uint32_t, hi);
+  if constexpr (PL == 2)
+    planes[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - float(hi[0]), b - float(hi[1])}, f16x2));
+}
+// Eight values as PL operand planes.
+template <int PL>
+__device__ __forceinline__ void split8(const f32x4 &a, const f32x4 &b, u32x4 (&planes)[PL]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    float a = x[i], b = x[i + 1];
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[PL];
+    if (i < 2) split2<PL>(a[2 * i], a[2 * i + 1], w);
+    else split2<PL>(b[2 * i - 4], b[2 * i - 3], w);
 #pragma unroll
-    for (int p = 0; p < PL; ++p) {
-      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-      planes[p][i / 2] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-      if (p + 1 < PL) {
-        a -= __uint_as_float(ua & 0xffff0000u);
-        b -= __uint_as_float(ub & 0xffff0000u);
-      }
-    }
+    for (int p = 0; p < PL; ++p) planes[p][i] = w[p];
   }
 }
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 // Sum of the plane products that count.
 template <int PA, int PB>
 __device__ __forceinline__ f32x4 mfma_planes(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x4 c) {
 #pragma unroll
-  for (int sum = 2; sum >= 0; --sum)  // small terms first
+  for (int i = 0; i < PA; ++i)
 #pragma unroll
-    for (int i = 0; i < PA; ++i)
-      if (sum - i >= 0 && sum - i < PB) c = mfma(a[i], b[sum - i], c);
+    for (int j = 0; j < PB; ++j)
+      if (i + j < 2) c = mfma(a[i], b[j], c);
   return c;
 }
 
-// Eight elements of a row of K or Q as planes (lane: row lane % 16, columns
-// from (lane / 16) * 8 of a 32-column step).
-template <typename A, int PL>
-__device__ __forceinline__ void load_planes(const A *row, bool live, int k0, int K, u32x4 (&planes)[PL]) {
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  if (live && k0 + 8 <= K) {
-    A raw[8];
-    __builtin_memcpy(raw, row + k0, sizeof(raw));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = to_f32(raw[e]);
-  } else if (live) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k0 + e < K) x[e] = to_f32(row[k0 + e]);
-  }
-  uint32_t w[PL][4];
-  split<PL, 8>(x, w);
-#pragma unroll
-  for (int p = 0; p < PL; ++p) planes[p] = u32x4{w[p][0], w[p][1], w[p][2], w[p][3]};
-}
-
-template <int PL>
-__device__ __forceinline__ float squares(const u32x4 (&planes)[PL]) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float lo = 0.0f, hi = 0.0f;
-#pragma unroll
-    for (int p = PL - 1; p >= 0; --p) {
-      lo += __uint_as_float(planes[p][i] << 16);
-      hi += __uint_as_float(planes[p][i] & 0xffff0000u);
-    }
-    s = fmaf(lo, lo, fmaf(hi, hi, s));
-  }
-  return s;
-}
-// Sum over lanes l, l ^ 16, l ^ 32, l ^ 48.
+// Sum / largest of lanes l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float sum_quarters(float x) {
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
   const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
+__device__ __forceinline__ float max_quarters(float x) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+// The largest of m and the values' magnitudes. Written out: fmaxf would first
+// quiet every operand in an instruction of its own.
+__device__ __forceinline__ float largest(float m, const f32x4 &x) {
+  asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(x[0]), "v"(x[1]));
+  asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(x[2]), "v"(x[3]));
+  return m;
+}
+// 2^-floor(log2 x) as a float (1 for 0, infinities and NaN), clamped so that it
+// and its inverse are normal numbers.
+__device__ __forceinline__ float inverse_power(float x) {
+  const int e = int((__float_as_uint(x) >> 23) & 0xffu);
+  const int c = e < 27 ? 27 : e > 227 ? 227 : e;
+  return e == 0xff || x == 0.0f ? 1.0f : __uint_as_float(uint32_t(254 - c) << 23);
+}
+
+// Inclusive sum over the wave's lanes in 64 bits.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xF, true));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xF, true));
+  return x + __builtin_bit_cast(double, (uint64_t(hi) << 32) | lo);
+}
+__device__ __forceinline__ double wave_prefix(double x) {
+  x = dpp_add64<0x111, 0xF>(x);  // row_shr 1, 2, 4, 8: sums inside 16 lanes
+  x = dpp_add64<0x112, 0xF>(x);
+  x = dpp_add64<0x114, 0xF>(x);
+  x = dpp_add64<0x118, 0xF>(x);
+  x = dpp_add64<0x142, 0xA>(x);  // row_bcast 15 into rows 1 and 3
+  return dpp_add64<0x143, 0xC>(x);  // row_bcast 31 into rows 2 and 3
+}
 
 // ---------------------------------------------------------------------------
-// Prepare: one workgroup per (slot, key head); the head's value heads in turn.
-// Wave w holds token rows 16w .. 16w + 15 of K K^T and Q K^T.
+// Prepare: one workgroup of four waves per (slot, value head); the first of a
+// key head's value heads also packs K, Q and K^T. Wave w holds token rows 16w
+// .. 16w + 15 of K K^T and Q K^T.
 // ---------------------------------------------------------------------------
-template <typename A, int PL, int OPL, int KP, bool PACK>
-__global__ __launch_bounds__(kPrefillThreads) void prepare_kernel(const PrefillArgs a) {
-  constexpr int KS = KP / 32, LD = kChunk + 4;
-  __shared__ float Ls[kChunk][LD], Ps[kChunk][LD];
-  __shared__ float rks[kChunk], rqs[kChunk];
+constexpr int kPrepareThreads = 256;
+
+// The lane's eight columns of a token row in operand order.
+template <typename A>
+__device__ __forceinline__ void load_row8(const A *row, bool live, int k0, int K, f32x4 (&x)[2]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int k = k0 + 16 * half;
+    x[half] = f32x4{0, 0, 0, 0};
+    if (live && k < K) {  // K is a multiple of 4
+      A raw[4];
+      __builtin_memcpy(raw, row + k, sizeof(raw));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[half][e] = to_f32(raw[e]);
+    }
+  }
+}
+
+constexpr int prepare_waves(int pl, int kp) { return pl == 1 && kp <= 128 ? 4 : pl == 1 || kp <= 128 ? 2 : 1; }
+
+template <typename A, typename Out, int KP>
+__global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)) void prepare_kernel(const PrefillArgs a) {
+  using U = Units<A, Out, KP>;
+  constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, LD = kChunk + 4;
+  constexpr int kLower = kChunk * LD * 4, kKeys = U::Q * kUnit;
+  __shared__ __attribute__((aligned(16))) char lds[kLower > kKeys ? kLower : kKeys];
+  __shared__ float kmul[kChunk], qmul[kChunk];  // what a row of K and Q was divided by, times the L2 norm's factor
+  float(*const Ls)[LD] = reinterpret_cast<float(*)[LD]>(lds);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  const int slot = int(blockIdx.x / unsigned(a.H)), h = int(blockIdx.x % unsigned(a.H));
+  const int slot = int(blockIdx.x / unsigned(a.HV)), hv = int(blockIdx.x % unsigned(a.HV));
+  const int h = hv / a.ratio;
+  const bool packs = hv % a.ratio == 0;
   const int b = __builtin_amdgcn_readfirstlane(
-      last_not_above(int(a.pages.rows), slot, [&](int i) { return first_slot(a, i); }));
+      last_not_above(int(a.pages.rows), slot, [&](int i) {
+        const int64_t at = load_index(a.pages.query_start_loc, i * a.pages.qsl_stride, a.pages.qsl_dtype);
+        return slot_of(a, i, clamp_token(at, a.pages.tokens));
+      }));
   if (b < 0) return;
   const Row r = load_row(a.pages, b);
   if (r.n == 0 || !r.valid) return;
   // The chunk's tokens.
   const int64_t C = a.align ? r.C : 0;
-  const int64_t o = (C / a.block) * a.per_block + (C % a.block) / kChunk + (slot - first_slot(a, b));
+  const int64_t o = (C / a.block) * a.per_block + (C % a.block) / kChunk + (slot - slot_of(a, b, r.bos));
   const int64_t blk = o / a.per_block;
   int64_t p0 = blk * a.block + (o % a.per_block) * kChunk, p1 = p0 + kChunk;
   p1 = p1 < (blk + 1) * a.block ? p1 : (blk + 1) * a.block;
@@ -185,38 +239,71 @@ __global__ __launch_bounds__(kPrefillThreads) void prepare_kernel(const PrefillA
   if (p0 >= p1) return;
   const int t0 = r.bos + int(p0 - C), n = int(p1 - p0);
 
-  const A *const kp = static_cast<const A *>(a.k) + int64_t(t0) * a.k_ts + int64_t(h) * a.K;
-  const A *const qp = static_cast<const A *>(a.q) + int64_t(t0) * a.q_ts + int64_t(h) * a.K;
-  const int64_t sh = int64_t(slot) * a.H + h;
+  // Gates, lane = token.
+  const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
+  float g = 0.0f, beta = 0.0f;
+  if (lane < n) {
+    g = load_as_f32(a.g, int64_t(t0 + lane) * a.g_ts + hv, a.g_dt);
+    beta = load_as_f32(a.beta, int64_t(t0 + lane) * a.beta_ts + hv, a.beta_dt);
+  }
 
+  // K and Q rows of this wave, scaled by powers of two.
   f32x4 kk[4], qk[4];
+  const int row = 16 * w + lr;
+  char *const key_ws = a.ws + (int64_t(slot) * a.H + h) * (U::KEY * kUnit);
   {
-    u32x4 kf[KS][PL], qf[KS][PL];
-    const int row = 16 * w + lr;
-    float ksq = 0.0f, qsq = 0.0f;
+    const A *const kp = static_cast<const A *>(a.k) + int64_t(t0 + row) * a.k_ts + int64_t(h) * a.K;
+    const A *const qp = static_cast<const A *>(a.q) + int64_t(t0 + row) * a.q_ts + int64_t(h) * a.K;
+    f32x4 kx[KS][2], qx[KS][2];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      load_planes<A, PL>(kp + row * a.k_ts, row < n, 32 * ks + 8 * lq, a.K, kf[ks]);
-      load_planes<A, PL>(qp + row * a.q_ts, row < n, 32 * ks + 8 * lq, a.K, qf[ks]);
-      if (a.l2norm) {
-        ksq += squares<PL>(kf[ks]);
-        qsq += squares<PL>(qf[ks]);
-      }
-      if constexpr (PACK) {
-        const int64_t at = (sh * 4 * KS * PL + (w * KS + ks) * PL) * kFrag + lane * 16;
+      load_row8(kp, row < n, 32 * ks + 4 * lq, a.K, kx[ks]);
+      load_row8(qp, row < n, 32 * ks + 4 * lq, a.K, qx[ks]);
+    }
+    float kmax = 0.0f, qmax = 0.0f;
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          *reinterpret_cast<u32x4 *>(a.ws + a.k_at + at + p * kFrag) = kf[ks][p];
-          *reinterpret_cast<u32x4 *>(a.ws + a.q_at + at + p * kFrag) = qf[ks][p];
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        kmax = fmaxf(kmax, fabsf(kx[ks][i >> 2][i & 3]));
+        qmax = fmaxf(qmax, fabsf(qx[ks][i >> 2][i & 3]));
+      }
+    const float kdiv = inverse_power(max_quarters(kmax)), qdiv = inverse_power(max_quarters(qmax));
+    float ksq = 0.0f, qsq = 0.0f;
+    u32x4 kf[KS][PL], qf[KS][PL];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float kv = kx[ks][i >> 2][i & 3] * kdiv, qv = qx[ks][i >> 2][i & 3] * qdiv;
+        kx[ks][i >> 2][i & 3] = kv;
+        qx[ks][i >> 2][i & 3] = qv;
+        ksq = fmaf(kv, kv, ksq);
+        qsq = fmaf(qv, qv, qsq);
+      }
+      split8<PL>(kx[ks][0], kx[ks][1], kf[ks]);
+      split8<PL>(qx[ks][0], qx[ks][1], qf[ks]);
+#pragma unroll
+      for (int p = 0; p < PL; ++p) {
+        const int at = ((w * KS + ks) * PL + p) * kUnit + lane * 16;
+        *reinterpret_cast<u32x4 *>(lds + at) = kf[ks][p];
+        if (packs) {
+          *reinterpret_cast<u32x4 *>(key_ws + at) = kf[ks][p];
+          *reinterpret_cast<u32x4 *>(key_ws + U::Q * kUnit + at) = qf[ks][p];
         }
       }
     }
-    ksq = sum_quarters(ksq);
-    qsq = sum_quarters(qsq);
-    if (lq == 0) {
-      rks[row] = a.l2norm ? 1.0f / sqrtf(ksq + 1e-6f) : 1.0f;
-      rqs[row] = a.l2norm ? 1.0f / sqrtf(qsq + 1e-6f) : 1.0f;
+    // With x' = x div and div a power of two, x / sqrt(|x|^2 + 1e-6) =
+    // x' / sqrt(|x'|^2 + 1e-6 div^2).
+    if (a.l2norm) {
+      ksq = sum_quarters(ksq);
+      qsq = sum_quarters(qsq);
     }
+    if (lq == 0) {
+      kmul[row] = a.l2norm ? 1.0f / sqrtf(ksq + 1e-6f * kdiv * kdiv) : 1.0f / kdiv;
+      qmul[row] = a.l2norm ? 1.0f / sqrtf(qsq + 1e-6f * qdiv * qdiv) : 1.0f / qdiv;
+    }
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       kk[j] = f32x4{0, 0, 0, 0};
@@ -225,88 +312,86 @@ __global__ __launch_bounds__(kPrefillThreads) void prepare_kernel(const PrefillA
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           u32x4 kb[PL];
-          load_planes<A, PL>(kp + (16 * j + lr) * a.k_ts, 16 * j + lr < n, 32 * ks + 8 * lq, a.K, kb);
+#pragma unroll
+          for (int p = 0; p < PL; ++p)
+            kb[p] = *reinterpret_cast<const u32x4 *>(lds + ((j * KS + ks) * PL + p) * kUnit + lane * 16);
           kk[j] = mfma_planes<PL, PL>(kf[ks], kb, kk[j]);
           qk[j] = mfma_planes<PL, PL>(qf[ks], kb, qk[j]);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          Ls[16 * w + lq * 4 + i][16 * j + lr] = 0.0f;
-          Ps[16 * w + lq * 4 + i][16 * j + lr] = 0.0f;
-        }
       }
     }
   }
-  // K^T in operand order: column 16 kt + lane % 16 of K, eight tokens a lane.
-  for (int f = w; f < KP / 16 * 2; f += 4) {
-    const int kc = (f >> 1) * 16 + lr, s0 = (f & 1) * 32 + lq * 8;
-    float x[8];
+  // K^T: column 16 i + lr of K, tokens in operand order.
+  if (packs) {
+    for (int f = w; f < KP / 8; f += 4) {
+      const int i = f >> 1, ts = f & 1;
+      // Element (token, column) lies in K's planes at token tile, columns / 32,
+      // lane (column % 16 / 4) * 16 + token % 16, half column % 32 / 16, place
+      // column % 4.
+      const int base = ((i >> 1) * PL) * kUnit + ((lr >> 2) * 16) * 16 + (i & 1) * 8 + (lr & 3) * 2;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = s0 + e < n && kc < a.K ? to_f32(kp[(s0 + e) * a.k_ts + kc]) : 0.0f;
-    uint32_t pl[PL][4];
-    split<PL, 8>(x, pl);
+      for (int p = 0; p < PL; ++p) {
+        u32x4 kt;
 #pragma unroll
-    for (int p = 0; p < PL; ++p)
-      *reinterpret_cast<u32x4 *>(a.ws + a.kt_at + ((sh * (KP / 8) + f) * PL + p) * kFrag + lane * 16) =
-          u32x4{pl[p][0], pl[p][1], pl[p][2], pl[p][3]};
+        for (int e = 0; e < 8; e += 2) {
+          const int tile = 2 * ts + (e >> 2), t = 4 * lq + (e & 3);
+          const char *at = lds + base + (tile * KS * PL + p) * kUnit + t * 16;
+          kt[e / 2] = uint32_t(*reinterpret_cast<const uint16_t *>(at)) |
+                      uint32_t(*reinterpret_cast<const uint16_t *>(at + 16)) << 16;
+        }
+        *reinterpret_cast<u32x4 *>(key_ws + (U::KT + f * PL + p) * kUnit + lane * 16) = kt;
+      }
+    }
   }
   __syncthreads();
 
-  for (int m = 0; m < a.ratio; ++m) {
-    const int hv = h * a.ratio + m;
-    const int64_t svh = int64_t(slot) * a.HV + hv;
-    // Lane = token: gates and the cumulative log decay, summed in 64 bits and
-    // kept as two floats, so that differences keep FP32 precision however far
-    // the sum has gone.
-    const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
-    float g = 0.0f, beta = 0.0f;
-    if (lane < n) {
-      g = log_decay(gates, load_as_f32(a.g, int64_t(t0 + lane) * a.g_ts + hv, a.g_dt));
-      beta = beta_of(gates, load_as_f32(a.beta, int64_t(t0 + lane) * a.beta_ts + hv, a.beta_dt));
-      g = g < kMinLogDecay ? kMinLogDecay : g;
-    }
-    double G = g;
+  // The cumulative log decay (base 2), summed in 64 bits and kept as two
+  // floats, so that differences keep FP32 precision however far the sum goes.
+  g = log_decay(gates, g);
+  g = lane < n ? (g < kMinLogDecay ? kMinLogDecay : g) : 0.0f;
+  beta = lane < n ? beta_of(gates, beta) : 0.0f;
+  const double G = wave_prefix(double(g) * 1.4426950408889634);
+  const float Gh = float(G), Gl = float(G - double(Gh));
+  char *const value_ws = a.ws_value + (int64_t(slot) * a.HV + hv) * (U::VALUE * kUnit);
+  if (w == 0) {
+    const double end = __shfl(G, 63);
+    float *sc = reinterpret_cast<float *>(value_ws + U::SC * kUnit);
+    const float e = __builtin_amdgcn_exp2f(Gh + Gl);
+    // The outputs' own scale: a power of two near Q's row, so that P fits F16.
+    const float mul = 1.0f / inverse_power(qmul[lane] * a.scale);
+    sc[kScIn * 64 + lane] = e * kmul[lane];
+    sc[kScQ * 64 + lane] = e * (a.scale * qmul[lane] / mul);
+    sc[kScOut * 64 + lane] = __builtin_amdgcn_exp2f(float(end - G)) * kmul[lane];
+    sc[kScMul * 64 + lane] = mul;
+    sc[kScEnd * 64 + lane] = __builtin_amdgcn_exp2f(float(end));
+  }
+  // L and P, token rows 16w + 4 lq + i, columns 16j + lr.
+  float Ght[4], Glt[4], bt[4], qt[4];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double up = __shfl_up(G, d);
-      G += lane >= d ? up : 0.0;
-    }
-    const float Gh = float(G), Gl = float(G - double(Gh));
-    if (w == 0) {
-      const double end = __shfl(G, 63);
-      float *sc = reinterpret_cast<float *>(a.ws + a.s_at) + svh * kScalars;
-      sc[kScIn + lane] = expf(Gh + Gl) * rks[lane];
-      sc[kScQ + lane] = a.scale * expf(Gh + Gl) * rqs[lane];
-      sc[kScOut + lane] = expf(float(end - G)) * rks[lane];
-      if (lane == 0) sc[kScEnd] = expf(float(end));
-    }
-    // L and P, token rows 16w + 4 lq + i, columns 16j + lr.
-    float Ght[4], Glt[4], bt[4], rkt[4], rqt[4];
+  for (int i = 0; i < 4; ++i) {
+    const int t = 16 * w + 4 * lq + i;
+    Ght[i] = __shfl(Gh, t);
+    Glt[i] = __shfl(Gl, t);
+    bt[i] = __shfl(beta, t) * kmul[t];
+    const float qs = qmul[t] * a.scale;
+    qt[i] = qs * inverse_power(qs);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int s = 16 * j + lr;
+    const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s), km = kmul[s];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 16 * w + 4 * lq + i;
-      Ght[i] = __shfl(Gh, t);
-      Glt[i] = __shfl(Gl, t);
-      rkt[i] = rks[t];
-      bt[i] = __shfl(beta, t) * rkt[i];
-      rqt[i] = rqs[t] * a.scale;
+      const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghs) + (Glt[i] - Gls)) * km;
+      Ls[t][s] = s < t ? bt[i] * d * kk[j][i] : 0.0f;
+      qk[j][i] = s <= t ? qt[i] * d * qk[j][i] : 0.0f;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j > w) break;
-      const int s = 16 * j + lr;
-      const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s), rk = rks[s];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * w + 4 * lq + i;
-        const float d = expf((Ght[i] - Ghs) + (Glt[i] - Gls)) * rk;
-        Ls[t][s] = s < t ? bt[i] * d * kk[j][i] : 0.0f;
-        Ps[t][s] = s <= t ? rqt[i] * d * qk[j][i] : 0.0f;
-      }
-    }
-    wave_fence();
-    // The diagonal block's inverse, a column a lane: x_i = [i = c] - sum_m L_im x_m.
+  }
+  wave_fence();
+  // The diagonal block's inverse, a column a lane: x_i = [i = c] - sum_m L_im x_m.
+  f32x4 T[4];  // T[d]: block (w + d, w)
+  {
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -315,340 +400,480 @@ __global__ __launch_bounds__(kPrefillThreads) void prepare_kernel(const PrefillA
       for (int c = 0; c < i; ++c) s = fmaf(-Ls[16 * w + i][16 * w + c], x[c], s);
       x[i] = s;
     }
-    f32x4 T[4];  // T[d]: block (w + d, w)
 #pragma unroll
     for (int i = 0; i < 4; ++i) T[0][i] = lq == 0 ? x[i] : lq == 1 ? x[4 + i] : lq == 2 ? x[8 + i] : x[12 + i];
-    wave_fence();
+  }
+  wave_fence();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * w + lr] = T[0][i];
-    __syncthreads();
-    // Block column w downwards: T_iw = -T_ii sum_{m = w}^{i - 1} L_im T_mw.
-    // Step i of the FP32 instruction takes columns 4 lq + i, which is where the
-    // accumulator of the block before holds its rows: no value moves.
+  for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * w + lr] = T[0][i];
+  __syncthreads();
+  // Block column w downwards: T_iw = -T_ii sum_{m = w}^{i - 1} L_im T_mw. Step i
+  // of the FP32 instruction takes columns 4 lq + i, which is where the
+  // accumulator of the block before holds its rows: no value moves. Two
+  // accumulators, because a product waits for the one before it on its own.
 #pragma unroll
-    for (int d = 1; d < 4; ++d) {
-      const int i = w + d;
-      T[d] = f32x4{0, 0, 0, 0};
-      if (i < 4) {
-        f32x4 acc = {0, 0, 0, 0};
+  for (int d = 1; d < 4; ++d) {
+    const int i = w + d;
+    T[d] = f32x4{0, 0, 0, 0};
+    if (i < 4) {
+      f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int e = 0; e < d; ++e) {
-          const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * (w + e) + 4 * lq]);
+      for (int e = 0; e < d; ++e) {
+        const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * (w + e) + 4 * lq]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(l[k], T[e][k], acc, 0, 0, 0);
-        }
-        const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * i + 4 * lq]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) T[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[k], acc[k], T[d], 0, 0, 0);
+        for (int k = 0; k < 4; ++k)
+          acc[k & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[k], T[e][k], acc[k & 1], 0, 0, 0);
       }
+      const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * i + 4 * lq]);
+      acc[0] += acc[1];
+      acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 &to = k & 1 ? acc[1] : T[d];
+        to = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[k], acc[0][k], to, 0, 0, 0);
+      }
+      T[d] += acc[1];
     }
-    __syncthreads();
-    const float bs = __shfl(beta, 16 * w + lr);
+  }
+  __syncthreads();
+  const float bs = __shfl(beta, 16 * w + lr);
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-      if (w + d < 4)
+  for (int d = 0; d < 4; ++d)
+    if (w + d < 4)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) Ls[16 * (w + d) + 4 * lq + i][16 * w + lr] = T[d][i] * bs;
-    __syncthreads();
+      for (int i = 0; i < 4; ++i) Ls[16 * (w + d) + 4 * lq + i][16 * w + lr] = T[d][i] * bs;
+  __syncthreads();
+  // Rows of T, then of P, as operands.
+  const auto rows_out = [&](auto planes, int unit) {
+    constexpr int N = decltype(planes)::value;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      if (ks * 32 > 16 * w + 15) continue;  // above the diagonal: never read
-      float y[8], z[8];
+      if (ks == 1 && w < 2) continue;
+      u32x4 f[N];
+      split8<N>(*reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 4 * lq]),
+                *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 16 + 4 * lq]), f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = Ls[16 * w + lr][32 * ks + 8 * lq + e];
-        z[e] = Ps[16 * w + lr][32 * ks + 8 * lq + e];
-      }
-      uint32_t tp[kPlanesT][4], pp[OPL][4];
-      split<kPlanesT, 8>(y, tp);
-      split<OPL, 8>(z, pp);
-      const int64_t f = svh * 8 + 2 * w + ks;
-#pragma unroll
-      for (int p = 0; p < kPlanesT; ++p)
-        *reinterpret_cast<u32x4 *>(a.ws + a.t_at + (f * kPlanesT + p) * kFrag + lane * 16) =
-            u32x4{tp[p][0], tp[p][1], tp[p][2], tp[p][3]};
-#pragma unroll
-      for (int p = 0; p < OPL; ++p)
-        *reinterpret_cast<u32x4 *>(a.ws + a.p_at + (f * OPL + p) * kFrag + lane * 16) =
-            u32x4{pp[p][0], pp[p][1], pp[p][2], pp[p][3]};
+      for (int p = 0; p < N; ++p)
+        *reinterpret_cast<u32x4 *>(value_ws + (unit + lower_block(w, ks) * N + p) * kUnit + lane * 16) = f[p];
     }
-    __syncthreads();
-  }
+  };
+  rows_out(std::integral_constant<int, 2>{}, 0);
+  wave_fence();
+  // A wave's rows of T are its own from here: P takes their place.
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * j + lr] = qk[j][i];
+  wave_fence();
+  rows_out(std::integral_constant<int, OPL>{}, U::P);
 }
 
 // ---------------------------------------------------------------------------
-// Scan: one workgroup per (row, value head, 16 NV rows of V). Wave w takes
-// token rows 16w .. 16w + 15 of a chunk's products and key columns KP/4 * w ..
-// of the state, which it holds transposed (a lane: 4 neighbouring k of one v).
+// Scan: one wave per (row, value head, 16 columns of V), which holds the state
+// transposed (a lane: one column v, four neighbouring k of each 16). All
+// products of a chunk keep a column of V in one lane group, so a wave needs
+// nothing of another's. NW waves of one head share a workgroup for the sake of
+// what they read: operands go from memory to LDS once for all of them, a chunk
+// ahead (two buffers), without passing registers.
 // ---------------------------------------------------------------------------
-template <typename A, int PL, int OPL, int KP, int NV, bool PACK>
-__global__ __launch_bounds__(kPrefillThreads) void scan_kernel(const PrefillArgs a) {
-  constexpr int KS = KP / 32, KT = KP / 64, SLD = KP + 8, CLD = kChunk + 8;
-  __shared__ uint16_t Sb[3][16 * NV][SLD], Rb[3][16 * NV][CLD], Cb[OPL][16 * NV][CLD], Db[3][16 * NV][CLD];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Byte offsets of a chunk's tokens stay under kScanExtent (the host checks the
+// strides), the size of every resource here. A lane outside the tensor takes
+// kScanDead plus up to a chunk's tokens: past the extent, so its load reads zero
+// and its store goes nowhere.
+constexpr int kScanExtent = 0x3ff80000, kScanDead = 0x3ffffff0;
+constexpr int64_t kScanReach = 0x3ff00000 / (kChunk * 4);  // elements of a token's stride and width
+
+// 1 KB a wave from memory to LDS, four in a row: an instruction's offset counts
+// for both sides. No register is written; the compiler does not see the LDS
+// writes, whose readers wait at the workgroup's barrier.
+__device__ __forceinline__ void copy_units4(const char *src, uint32_t lane_at, uint32_t dst) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "global_load_lds_dwordx4 %0, %1\n\t"
+      "global_load_lds_dwordx4 %0, %1 offset:1024\n\t"
+      "global_load_lds_dwordx4 %0, %1 offset:2048\n\t"
+      "global_load_lds_dwordx4 %0, %1 offset:3072" ::"v"(lane_at),
+      "s"(src), "s"(dst));
+}
+__device__ __forceinline__ void copy_units2(const char *src, uint32_t lane_at, uint32_t dst) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "global_load_lds_dwordx4 %0, %1\n\t"
+      "global_load_lds_dwordx4 %0, %1 offset:1024" ::"v"(lane_at),
+      "s"(src), "s"(dst));
+}
+
+// Whether two chunks' operands fit LDS; else waves read them from memory.
+constexpr bool scan_staged(int pl, int opl, int kp) { return 2 * (12 * (kp / 32) * pl + 14 + 6 * opl) <= 160; }
+
+// At most 256 registers (two waves a SIMD), so that none are accumulation
+// registers, which every other instruction would have to copy from and to. LDS
+// is the launch's: told its size, the compiler would reckon with one wave.
+template <typename A, typename Out, int KP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
+  using U = Units<A, Out, KP>;
+  constexpr int PL = U::PL, OPL = U::OPL, ob = int(sizeof(Out));
+  constexpr bool STAGED = scan_staged(PL, OPL, KP);
+  constexpr int KS = KP / 32, NT = KP / 16, EB = int(sizeof(A)), UNITS = U::KEY + U::VALUE;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];  // STAGED: two chunks' operands
+  const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
-  // Workgroups of one key head's group (they read the same K, Q, T and P) sit
-  // on one XCD: consecutive workgroups go to the eight XCDs in turn.
+  // Workgroups of one key head's group (they read the same K and Q) sit on one
+  // XCD: consecutive workgroups go to the eight XCDs in turn.
   const int wg = int(blockIdx.x), group = (wg / 8 / a.members) * 8 + wg % 8, member = wg / 8 % a.members;
   if (group >= a.pages.rows * a.H) return;
   const int b = group / a.H, h = group % a.H;
-  const int hv = h * a.ratio + member / a.slices, v0 = member % a.slices * (16 * NV);
+  const int hv = h * a.ratio + member / a.slices, v0 = (member % a.slices * NW + wave) * 16;
   const Row r = load_row(a.pages, b);
   if (r.n == 0) return;
+  const bool column = v0 + lr < a.V;
   if (!r.valid) {
-    const int width = a.V - v0 < 16 * NV ? a.V - v0 : 16 * NV;
-    for (int64_t i = threadIdx.x; i < int64_t(r.n) * width; i += kPrefillThreads) {
-      const int64_t at = (r.bos + i / width) * a.out_ts + int64_t(hv) * a.V + v0 + i % width;
-      if (a.out_f32) static_cast<float *>(a.out)[at] = 0.0f;
-      else static_cast<A *>(a.out)[at] = from_f32<A>(0.0f);
+    for (int t = lq; t < r.n; t += 4) {
+      const int64_t at = int64_t(r.bos + t) * a.out_ts + int64_t(hv) * a.V + v0 + lr;
+      if (column) {
+        static_cast<Out *>(a.out)[at] = from_f32<Out>(0.0f);
+      }
     }
     return;
   }
-  const auto state_at = [&](int64_t page, int i, int nv) {  // element offset of the lane's four k
-    return page * a.state_bs + hv * a.state_hs + int64_t(v0 + 16 * nv + lr) * a.state_vs + 16 * (w * KT + i) + 4 * lq;
-  };
-  const auto state_live = [&](int i, int nv) { return v0 + 16 * nv + lr < a.V && 16 * (w * KT + i) + 4 * lq < a.K; };
-  const auto store_state = [&](int64_t page, const f32x4 (&S)[KT][NV]) {
-#pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
-        if (state_live(i, nv)) {
-          const int64_t at = state_at(page, i, nv);
-          if (a.state_dt == GDN_DT_F32) {
-            *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = S[i][nv];
-          } else if (a.state_dt == GDN_DT_BF16) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(S[i][nv][e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(S[i][nv][e]);
-          }
-        }
-  };
-  f32x4 S[KT][NV];
-#pragma unroll
-  for (int i = 0; i < KT; ++i)
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      S[i][nv] = f32x4{0, 0, 0, 0};
-      if (!r.fresh && state_live(i, nv))
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[i][nv][e] = load_as_f32(a.state, state_at(r.src, i, nv) + e, a.state_dt);
-    }
+  const int64_t slot = slot_of(a, b, r.bos);
+  const char *key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit);
+  const char *value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit);
+  const int64_t key_step = int64_t(a.H) * (U::KEY * kUnit), value_step = int64_t(a.HV) * (U::VALUE * kUnit);
+  const uint32_t lane_at = lane * 16;
 
-  int64_t slot = first_slot(a, b);
+  // Chunk lengths from position to position.
   int done = 0, inside = a.align ? int(r.C % a.block) : 0;
-  while (done < r.n) {
-    int n = kChunk - inside % kChunk;
-    n = n < a.block - inside ? n : a.block - inside;
-    n = n < r.n - done ? n : r.n - done;
-    const int t0 = r.bos + done;
-    const int64_t sh = slot * a.H + h, svh = slot * a.HV + hv;
-    const float *sc = reinterpret_cast<const float *>(a.ws + a.s_at) + svh * kScalars;
-    // The state, as planes, to every wave.
+  const auto length = [&](int at, int in) {
+    int n = kChunk - (in & (kChunk - 1));
+    n = n < a.block - in ? n : a.block - in;
+    return n < r.n - at ? n : r.n - at;
+  };
+  int n = length(0, inside);
+
+  // Operands of the current chunk, by unit.
+  int buffer = 0;
+  const auto operand = [&](int u) -> u32x4 {
+    if constexpr (STAGED) return *reinterpret_cast<const u32x4 *>(lds + buffer + u * kUnit + lane_at);
+    else return *reinterpret_cast<const u32x4 *>((u < U::KEY ? key_ws + u * kUnit : value_ws + (u - U::KEY) * kUnit) + lane_at);
+  };
+  const auto scalars = [&](int array, int tile) -> f32x4 {
+    const int at = array * 256 + (16 * tile + 4 * lq) * 4;
+    if constexpr (STAGED) return *reinterpret_cast<const f32x4 *>(lds + buffer + (U::KEY + U::SC) * kUnit + at);
+    else return *reinterpret_cast<const f32x4 *>(value_ws + U::SC * kUnit + at);
+  };
+  // The wave's jobs of four units each, of the chunk at (key, value).
+  constexpr int KEY_GROUPS = U::KEY / 4, GROUPS = KEY_GROUPS + (U::VALUE + 3) / 4, JOBS = (GROUPS + NW - 1) / NW;
+  const uint32_t lds_base = uint32_t(uintptr_t((__attribute__((address_space(3))) char *)lds));
+  const auto stage = [&](int from, int till, const char *key, const char *value, int to) {
+    if constexpr (STAGED) {
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        const float x[4] = {S[i][nv][0], S[i][nv][1], S[i][nv][2], S[i][nv][3]};
-        uint32_t pl[3][2];
-        split<3, 4>(x, pl);
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-          *reinterpret_cast<u32x2 *>(&Sb[p][16 * nv + lr][16 * (w * KT + i) + 4 * lq]) = u32x2{pl[p][0], pl[p][1]};
+      for (int j = 0; j < JOBS; ++j) {
+        if (j < from || j >= till) continue;
+        const int g = j * NW + wave;
+        const char *src = g < KEY_GROUPS ? key + g * 4 * kUnit : value + (g - KEY_GROUPS) * 4 * kUnit;
+        const uint32_t dst = lds_base + uint32_t(to + g * 4 * kUnit);
+        if (g < GROUPS - (U::VALUE % 4 == 2)) copy_units4(src, lane_at, dst);
+        else if (U::VALUE % 4 == 2 && g == GROUPS - 1) copy_units2(src, lane_at, dst);
       }
-    lds_barrier();
-    // X = K S0^T and Q S0^T.
-    f32x4 X[NV], O[NV];
+    }
+  };
+  stage(0, JOBS, key_ws, value_ws, 0);
+
+  // V of the chunk: rows past its n tokens lie behind the resource's end.
+  const int v_bytes = int(a.v_ts) * EB, out_bytes = int(a.out_ts) * ob;
+  const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + r.bos * a.v_ts + int64_t(hv) * a.V);
+  char *op = static_cast<char *>(a.out) + (r.bos * a.out_ts + int64_t(hv) * a.V) * ob;
+  const int v_col = column ? (v0 + lr) * EB + 4 * lq * v_bytes : kScanDead;
+  const int out_col = column ? (v0 + lr) * ob + 4 * lq * out_bytes : kScanDead;
+  uint32_t vv[4][4];
+  const auto load_v = [&](int tokens) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(vp), 0,
+                                                      tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0, 0x00020000);
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv) X[nv] = O[nv] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int off = v_col + (16 * t + i) * v_bytes;
+        if constexpr (EB == 4) vv[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+        else vv[t][i] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
+      }
+  };
+  const auto value = [&](int t, int i) {
+    if constexpr (EB == 4) return __uint_as_float(vv[t][i]);
+    else return to_f32(__builtin_bit_cast(A, uint16_t(vv[t][i])));
+  };
+  load_v(n);
+
+  const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
+    return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * i + 4 * lq;
+  };
+  f32x4 S[NT];
+  float sigma = 1.0f, unscale = 1.0f;  // S, v, c and out of this lane's column stand here times sigma
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    S[i] = f32x4{0, 0, 0, 0};
+    if (!r.fresh && column && 16 * i + 4 * lq < a.K)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
+  }
+  const auto store_state = [&](int64_t page) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      if (column && 16 * i + 4 * lq < a.K) {
+        const int64_t at = state_at(page, i);
+        const f32x4 x = S[i] * unscale;
+        if (a.state_dt == GDN_DT_F32) {
+          *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
+        } else if (a.state_dt == GDN_DT_BF16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+        }
+      }
+  };
+  const auto rescale = [&](float f) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) S[i] *= f;
+    sigma *= f;
+    unscale /= f;
+  };
+
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  while (true) {
+    if constexpr (STAGED) lds_barrier();
+    // The next chunk; where there is none, its loads repeat this one's slot and
+    // take no tokens.
+    const int done_next = done + n;
+    int in_next = inside + n;
+    in_next = in_next == a.block ? 0 : in_next;
+    const bool more = done_next < r.n;
+    const int n_next = more ? length(done_next, in_next) : 0;
+    const char *key_next = key_ws + (more ? key_step : 0), *value_next = value_ws + (more ? value_step : 0);
+    const int to = UNITS * kUnit - buffer;
+    vp += int64_t(n) * v_bytes;
+
+    // Keep this column's values inside F16: with |k| near 1, |S0 k| is at most
+    // sqrt(K) <= 16 times S0's largest element, and where the rule is stable the
+    // corrections stay under 64 times v's largest plus that.
+    {
+      float ms = 0.0f, mv = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) ms = largest(ms, S[i]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mv = largest(mv, f32x4{value(t, 0), value(t, 1), value(t, 2), value(t, 3)});
+      const float m = max_quarters(fmaxf(16.0f * ms, 64.0f * sigma * mv));
+      const bool fits = m == 0.0f || !(m < 64.0f || m > 16384.0f) || m > 3e38f;
+      if (__builtin_amdgcn_ballot_w64(!fits) != 0) rescale(fits ? 1.0f : 2048.0f * inverse_power(m));
+    }
+    // X = K S0^T and Q S0^T.
+    f32x4 X[4], O[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) X[t] = O[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      u32x4 kf[PL], qf[PL];
-      if constexpr (PACK) {
-        const int64_t at = (sh * 4 * KS * PL + (w * KS + ks) * PL) * kFrag + lane * 16;
+      u32x4 sp[2], so[OPL];
+      split8<2>(S[2 * ks], S[2 * ks + 1], sp);
+#pragma unroll
+      for (int p = 0; p < OPL; ++p) so[p] = sp[p];
+      u32x4 kf[4][PL], qf[4][PL];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int p = 0; p < PL; ++p) {
-          kf[p] = *reinterpret_cast<const u32x4 *>(a.ws + a.k_at + at + p * kFrag);
-          qf[p] = *reinterpret_cast<const u32x4 *>(a.ws + a.q_at + at + p * kFrag);
+          kf[t][p] = operand((t * KS + ks) * PL + p);
+          qf[t][p] = operand(U::Q + (t * KS + ks) * PL + p);
         }
-      } else {
-        const int row = 16 * w + lr;
-        const bool live = row < n && 32 * ks + 8 * lq < a.K;
-        kf[0] = qf[0] = u32x4{0, 0, 0, 0};
-        if (live) {
-          const A *kr = static_cast<const A *>(a.k) + int64_t(t0 + row) * a.k_ts + int64_t(h) * a.K + 32 * ks + 8 * lq;
-          const A *qr = static_cast<const A *>(a.q) + int64_t(t0 + row) * a.q_ts + int64_t(h) * a.K + 32 * ks + 8 * lq;
-          __builtin_memcpy(&kf[0], kr, 16);
-          __builtin_memcpy(&qf[0], qr, 16);
-        }
-      }
+      // Token tile by token tile for each pair of planes: a product waits for
+      // the one before it on its accumulator.
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        u32x4 s[3];
+      for (int i = 0; i < PL; ++i)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) s[p] = *reinterpret_cast<const u32x4 *>(&Sb[p][16 * nv + lr][32 * ks + 8 * lq]);
-        X[nv] = mfma_planes<PL, 3>(kf, s, X[nv]);
-        u32x4 so[OPL];
+        for (int j = 0; j < 2; ++j)
+          if (i + j < 2)
 #pragma unroll
-        for (int p = 0; p < OPL; ++p) so[p] = s[p];
-        O[nv] = mfma_planes<PL, OPL>(qf, so, O[nv]);
+            for (int t = 0; t < 4; ++t) X[t] = mfma(kf[t][i], sp[j], X[t]);
+#pragma unroll
+      for (int i = 0; i < PL; ++i)
+#pragma unroll
+        for (int j = 0; j < OPL; ++j)
+          if (i + j < 2)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) O[t] = mfma(qf[t][i], so[j], O[t]);
+      stage(JOBS * ks / KS, JOBS * (ks + 1) / KS, key_next, value_next, to);
+    }
+    // R = v - diag(e^G) X.
+    f32x4 R[4];
+    float mr = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 in = scalars(kScIn, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) R[t][i] = fmaf(-in[i], X[t][i], sigma * value(t, i));
+      mr = largest(mr, R[t]);
+    }
+    load_v(n_next);
+    if (__builtin_amdgcn_ballot_w64(mr > 32768.0f) != 0) {
+      const float m = max_quarters(mr), f = m > 32768.0f ? 2048.0f * inverse_power(m) : 1.0f;
+      rescale(f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        R[t] *= f;
+        O[t] *= f;
       }
     }
-    // R = V - diag(e^G) X.
-    const f32x4 in = *reinterpret_cast<const f32x4 *>(sc + kScIn + 16 * w + 4 * lq);
-#pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      float x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * w + 4 * lq + i, v = v0 + 16 * nv + lr;
-        const float vv =
-            t < n && v < a.V ? to_f32(static_cast<const A *>(a.v)[int64_t(t0 + t) * a.v_ts + int64_t(hv) * a.V + v]) : 0.0f;
-        x[i] = t < n ? fmaf(-in[i], X[nv][i], vv) : 0.0f;
-      }
-      uint32_t pl[3][2];
-      split<3, 4>(x, pl);
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<u32x2 *>(&Rb[p][16 * nv + lr][16 * w + 4 * lq]) = u32x2{pl[p][0], pl[p][1]};
-    }
-    lds_barrier();
     // c = T R.
-    f32x4 Cc[NV];
+    f32x4 c[4];
+    {
+      u32x4 rp[2][2];
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv) Cc[nv] = f32x4{0, 0, 0, 0};
+      for (int ks = 0; ks < 2; ++ks) split8<2>(R[2 * ks], R[2 * ks + 1], rp[ks]);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks * 32 > 16 * w + 15) continue;
-      u32x4 tf[kPlanesT];
+      for (int t = 0; t < 4; ++t) c[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int p = 0; p < kPlanesT; ++p)
-        tf[p] = *reinterpret_cast<const u32x4 *>(a.ws + a.t_at + ((svh * 8 + 2 * w + ks) * kPlanesT + p) * kFrag + lane * 16);
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 tf[4][2];
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        u32x4 rf[3];
+        for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) rf[p] = *reinterpret_cast<const u32x4 *>(&Rb[p][16 * nv + lr][32 * ks + 8 * lq]);
-        Cc[nv] = mfma_planes<kPlanesT, 3>(tf, rf, Cc[nv]);
+          for (int p = 0; p < 2; ++p) tf[t][p] = operand(U::KEY + lower_block(t, ks) * 2 + p);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (i + j < 2)
+#pragma unroll
+              for (int t = 2 * ks; t < 4; ++t) c[t] = mfma(tf[t][i], rp[ks][j], c[t]);
       }
     }
-    const f32x4 decay = *reinterpret_cast<const f32x4 *>(sc + kScOut + 16 * w + 4 * lq);
+    // d = diag(e^{G_end - G}) c.
+    f32x4 d[4];
+    float mc = 0.0f;
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv) {
-      float x[4], y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = Cc[nv][i];
-        y[i] = x[i] * decay[i];
-      }
-      uint32_t pc[OPL][2], pd[3][2];
-      split<OPL, 4>(x, pc);
-      split<3, 4>(y, pd);
-#pragma unroll
-      for (int p = 0; p < OPL; ++p)
-        *reinterpret_cast<u32x2 *>(&Cb[p][16 * nv + lr][16 * w + 4 * lq]) = u32x2{pc[p][0], pc[p][1]};
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<u32x2 *>(&Db[p][16 * nv + lr][16 * w + 4 * lq]) = u32x2{pd[p][0], pd[p][1]};
+    for (int t = 0; t < 4; ++t) {
+      d[t] = c[t] * scalars(kScOut, t);
+      mc = largest(largest(mc, c[t]), d[t]);
     }
-    lds_barrier();
-    // S1 = e^{G_end} S0 + K^T (diag(e^{G_end - G}) c).
-    const float end = sc[kScEnd];
+    if (__builtin_amdgcn_ballot_w64(mc > 32768.0f) != 0) {
+      const float m = max_quarters(mc), f = m > 32768.0f ? 2048.0f * inverse_power(m) : 1.0f;
+      rescale(f);
 #pragma unroll
-    for (int i = 0; i < KT; ++i)
+      for (int t = 0; t < 4; ++t) {
+        c[t] *= f;
+        d[t] *= f;
+        O[t] *= f;
+      }
+    }
+    // S1 = e^{G_end} S0 + K^T d.
+    const float end = scalars(kScEnd, 0)[0];
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) S[i][nv] *= end;
+    for (int i = 0; i < NT; ++i) S[i] *= end;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      u32x4 df[NV][3];
+      u32x4 dp[2];
+      split8<2>(d[2 * ks], d[2 * ks + 1], dp);
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv)
+      for (int i0 = 0; i0 < NT; i0 += 4) {
+        u32x4 kt[4][PL];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) df[nv][p] = *reinterpret_cast<const u32x4 *>(&Db[p][16 * nv + lr][32 * ks + 8 * lq]);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        u32x4 kt[PL];
+          for (int p = 0; p < PL; ++p) kt[i][p] = operand(U::KT + ((i0 + i) * 2 + ks) * PL + p);
 #pragma unroll
-        for (int p = 0; p < PL; ++p)
-          kt[p] = *reinterpret_cast<const u32x4 *>(
-              a.ws + a.kt_at + ((sh * (KP / 8) + (w * KT + i) * 2 + ks) * PL + p) * kFrag + lane * 16);
+        for (int x = 0; x < PL; ++x)
 #pragma unroll
-        for (int nv = 0; nv < NV; ++nv) S[i][nv] = mfma_planes<PL, 3>(kt, df[nv], S[i][nv]);
+          for (int y = 0; y < 2; ++y)
+            if (x + y < 2)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) S[i0 + i] = mfma(kt[i][x], dp[y], S[i0 + i]);
       }
     }
     // out = diag(scale e^G) Q S0^T + P c.
-    const f32x4 oq = *reinterpret_cast<const f32x4 *>(sc + kScQ + 16 * w + 4 * lq);
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv) O[nv] *= oq;
+    for (int t = 0; t < 4; ++t) O[t] *= scalars(kScQ, t);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      if (ks * 32 > 16 * w + 15) continue;
-      u32x4 pf[OPL];
+      u32x4 cp[OPL], pf[4][OPL];
+      split8<OPL>(c[2 * ks], c[2 * ks + 1], cp);
 #pragma unroll
-      for (int p = 0; p < OPL; ++p)
-        pf[p] = *reinterpret_cast<const u32x4 *>(a.ws + a.p_at + ((svh * 8 + 2 * w + ks) * OPL + p) * kFrag + lane * 16);
+      for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
-      for (int nv = 0; nv < NV; ++nv) {
-        u32x4 cf[OPL];
+        for (int p = 0; p < OPL; ++p) pf[t][p] = operand(U::KEY + U::P + lower_block(t, ks) * OPL + p);
 #pragma unroll
-        for (int p = 0; p < OPL; ++p) cf[p] = *reinterpret_cast<const u32x4 *>(&Cb[p][16 * nv + lr][32 * ks + 8 * lq]);
-        O[nv] = mfma_planes<OPL, OPL>(pf, cf, O[nv]);
-      }
+      for (int i = 0; i < OPL; ++i)
+#pragma unroll
+        for (int j = 0; j < OPL; ++j)
+          if (i + j < 2)
+#pragma unroll
+            for (int t = 2 * ks; t < 4; ++t) O[t] = mfma(pf[t][i], cp[j], O[t]);
     }
+    // What was loaded for the next chunk is here; this chunk's stores then have
+    // that chunk's time.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(op, 0, (n - 1) * out_bytes + a.V * ob, 0x00020000);
 #pragma unroll
-    for (int nv = 0; nv < NV; ++nv)
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 x = O[t] * (scalars(kScMul, t) * unscale);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * w + 4 * lq + i, v = v0 + 16 * nv + lr;
-        if (t < n && v < a.V) {
-          const int64_t at = int64_t(t0 + t) * a.out_ts + int64_t(hv) * a.V + v;
-          if (a.out_f32) static_cast<float *>(a.out)[at] = O[nv][i];
-          else static_cast<A *>(a.out)[at] = from_f32<A>(O[nv][i]);
+        for (int i = 0; i < 4; ++i) {
+          const int off = out_col + (16 * t + i) * out_bytes;
+          if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, off, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, off, 0, 0);
         }
       }
-    done += n;
-    inside += n;
-    ++slot;
-    if (inside == a.block) {
-      inside = 0;
-      if (a.align && done < r.n) {
-        const int64_t page = boundary_page(a.pages, r, r.C + done);
-        if (page != 0) store_state(page, S);
-      }
+      op += int64_t(n) * out_bytes;
     }
+    if (!more) break;
+    if (a.align && in_next == 0) {
+      const int64_t page = boundary_page(a.pages, r, r.C + done_next);
+      if (page != 0) store_state(page);
+    }
+    key_ws = key_next;
+    value_ws = value_next;
+    buffer = to;
+    done = done_next;
+    inside = in_next;
+    n = n_next;
   }
-  store_state(r.fin, S);
+  store_state(r.fin);
 }
 
-template <typename A, int PL, int OPL, bool PACK, int KP>
-static void launch_prefill_dims(int nv, unsigned scan_grid, hipStream_t s, const PrefillArgs &a) {
-  hipLaunchKernelGGL((prepare_kernel<A, PL, OPL, KP, PACK>), dim3(unsigned(a.slots) * unsigned(a.H)),
-                     dim3(kPrefillThreads), 0, s, a);
-  if (nv == 1)
-    hipLaunchKernelGGL((scan_kernel<A, PL, OPL, KP, 1, PACK>), dim3(scan_grid), dim3(kPrefillThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((scan_kernel<A, PL, OPL, KP, 2, PACK>), dim3(scan_grid), dim3(kPrefillThreads), 0, s, a);
+template <typename A, typename Out, int KP, int NW>
+static void launch_scan(unsigned grid, hipStream_t s, const PrefillArgs &a) {
+  using U = Units<A, Out, KP>;
+  const unsigned lds = scan_staged(U::PL, U::OPL, KP) ? 2 * (U::KEY + U::VALUE) * kUnit : 0;
+  hipLaunchKernelGGL((scan_kernel<A, Out, KP, NW>), dim3(grid), dim3(64 * NW), lds, s, a);
 }
-template <typename A, int PL, int OPL, bool PACK>
-void launch_prefill(int kp, int nv, unsigned scan_grid, hipStream_t s, const PrefillArgs &a);
-
-#define GDN_PREFILL(A, PL, OPL, PACK)                                                                            \
-  template <>                                                                                                    \
-  void launch_prefill<A, PL, OPL, PACK>(int kp, int nv, unsigned grid, hipStream_t s, const PrefillArgs &a) {    \
-    if (kp == 64) launch_prefill_dims<A, PL, OPL, PACK, 64>(nv, grid, s, a);                                     \
-    else if (kp == 128) launch_prefill_dims<A, PL, OPL, PACK, 128>(nv, grid, s, a);                              \
-    else launch_prefill_dims<A, PL, OPL, PACK, 256>(nv, grid, s, a);                                             \
+template <typename A, typename Out, int KP>
+static void launch_prefill_dims(int nw, unsigned scan_grid, hipStream_t s, const PrefillArgs &a) {
+  hipLaunchKernelGGL((prepare_kernel<A, Out, KP>), dim3(unsigned(a.slots) * unsigned(a.HV)), dim3(kPrepareThreads), 0, s, a);
+  if constexpr (scan_staged(key_planes<A>(), out_planes<Out>(), KP)) {
+    if (nw == 1) return launch_scan<A, Out, KP, 1>(scan_grid, s, a);
+    if (nw == 2) return launch_scan<A, Out, KP, 2>(scan_grid, s, a);
+    if (nw == 8) return launch_scan<A, Out, KP, 8>(scan_grid, s, a);
   }
-#define GDN_PREFILL_DECL(A, PL, OPL, PACK) \
-  template <>                              \
-  void launch_prefill<A, PL, OPL, PACK>(int, int, unsigned, hipStream_t, const PrefillArgs &);
-GDN_PREFILL_DECL(bf16, 1, 2, false)
-GDN_PREFILL_DECL(bf16, 2, 2, true)
-GDN_PREFILL_DECL(bf16, 3, 3, true)
-GDN_PREFILL_DECL(f16, 2, 2, true)
-GDN_PREFILL_DECL(f16, 3, 3, true)
-GDN_PREFILL_DECL(float, 3, 3, true)
+  launch_scan<A, Out, KP, 4>(scan_grid, s, a);
+}
+template <typename A, typename Out>
+void launch_prefill(int kp, int nw, unsigned scan_grid, hipStream_t s, const PrefillArgs &a);
+
+#define GDN_PREFILL(A, Out)                                                                         \
+  template <>                                                                                     \
+  void launch_prefill<A, Out>(int kp, int nw, unsigned grid, hipStream_t s, const PrefillArgs &a) { \
+    if (kp == 64) launch_prefill_dims<A, Out, 64>(nw, grid, s, a);                                  \
+    else if (kp == 128) launch_prefill_dims<A, Out, 128>(nw, grid, s, a);                           \
+    else launch_prefill_dims<A, Out, 256>(nw, grid, s, a);                                          \
+  }
+#define GDN_PREFILL_DECL(A, Out) \
+  template <>                  \
+  void launch_prefill<A, Out>(int, int, unsigned, hipStream_t, const PrefillArgs &);
+GDN_PREFILL_DECL(bf16, bf16)
+GDN_PREFILL_DECL(bf16, float)
+GDN_PREFILL_DECL(f16, f16)
+GDN_PREFILL_DECL(f16, float)
+GDN_PREFILL_DECL(float, float)
 
 }  // namespace gdn

@@ -21,6 +21,15 @@ __device__ __forceinline__ int clamp_token(int64_t t, int64_t tokens) {
   return int(t < 0 ? 0 : t > tokens ? tokens : t);
 }
 
+// A wave-uniform 64-bit value in scalar registers: 64-bit compares and what
+// hangs on them are vector instructions, and a buffer address made by those
+// costs a loop at every access.
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(uint64_t(x)))));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(uint64_t(x) >> 32))));
+  return int64_t((uint64_t(hi) << 32) | lo);
+}
+
 // The row's words are read at wave-uniform addresses: the four that depend on
 // nothing are in flight together, the block table's entry follows.
 __device__ __forceinline__ Row load_row(const gdn_row_pages &p, int b) {
@@ -54,6 +63,14 @@ __device__ __forceinline__ Row load_row(const gdn_row_pages &p, int b) {
     r.fin = load_index_ro(p.final_indices, b * p.final_stride, p.final_dtype);
   }
   r.valid = r.valid && r.fin > 0 && r.fin < p.blocks && (r.fresh || (r.src > 0 && r.src < p.blocks));
+  r.bos = __builtin_amdgcn_readfirstlane(r.bos);
+  r.n = __builtin_amdgcn_readfirstlane(r.n);
+  r.C = uniform64(r.C);
+  r.req = uniform64(r.req);
+  r.src = uniform64(r.src);
+  r.fin = uniform64(r.fin);
+  r.fresh = __builtin_amdgcn_readfirstlane(int(r.fresh)) != 0;
+  r.valid = __builtin_amdgcn_readfirstlane(int(r.valid)) != 0;
   return r;
 }
 
