@@ -1,5 +1,6 @@
 // C entry points of the chunked gated delta rule: checks, workspace, dispatch
 // (kernels in prefill_kernel.cuh, instantiated in prefill_*.hip).
+#include <cstdlib>
 #include "prefill_kernel.cuh"
 
 namespace gdn {
@@ -35,21 +36,20 @@ static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &
       return false;
     }
   }
-  // A row of n tokens spans at most n * per_block / block + 3 chunks wherever it
-  // starts, and ceil(n / 64) where chunks start with the row.
   a.align = rp.block_table != nullptr;
   a.block = a.align ? int32_t(rp.block_size) : kChunk;
   a.per_block = (a.block + kChunk - 1) / kChunk;
-  a.slack = a.align ? 3 : 1;
-  const int64_t slots = rp.tokens * a.per_block / a.block + a.slack * rp.rows;
+  const int64_t slots = slot_of(a.align, a.block, int(rp.rows), int(rp.tokens));
   p.kp = K <= 64 ? 64 : K <= 128 ? 128 : 256;
   p.pl = l->act_dtype == GDN_DT_F32 ? 2 : 1;
   p.opl = l->act_dtype == GDN_DT_BF16 && !a.out_f32 ? 1 : 2;
   p.key_bytes = slots * H * (12 * (p.kp / 32) * p.pl) * kUnit;
   p.bytes = p.key_bytes + slots * HV * (14 + 6 * p.opl) * kUnit;
   const int64_t tiles = rp.rows * HV * ((V + 15) / 16);
-  p.nw = !scan_staged(p.pl, p.opl, p.kp) ? 4 : tiles <= 256 ? 1 : tiles <= 512 ? 2 : tiles <= 1024 ? 4 : 8;
-  a.slices = int32_t((V + 16 * p.nw - 1) / (16 * p.nw));
+  p.nw = tiles <= 1024 ? 0 : !scan_staged(p.pl, p.opl, p.kp) ? 4 : 8;
+  if (const char *e = getenv("PF_NW")) p.nw = atoi(e);
+  const int per = 16 * (p.nw ? p.nw : 1);
+  a.slices = int32_t((V + per - 1) / per);
   a.members = a.ratio * a.slices;
   p.scan_grid = (rp.rows * H + 7) / 8 * 8 * a.members;
   if (slots * HV > 0x7fffffffLL || p.scan_grid > 0x7fffffffLL || rp.rows * H > 0x7fffffffLL) {

@@ -57,9 +57,8 @@ struct PrefillArgs {
   int32_t g_dt, beta_dt, state_dt, out_f32, gated, l2norm;
   float scale;
   // Chunk geometry: positions are cut at multiples of 64 inside blocks of
-  // `block` tokens, per_block chunks each; row b's chunks start at slot
-  // qsl[b] * per_block / block + slack * b, which leaves every row enough.
-  int32_t align, block, per_block, slack, slots;
+  // `block` tokens, per_block chunks each.
+  int32_t align, block, per_block, slots;
   char *ws;        // per (slot, key head): K, Q, K^T
   char *ws_value;  // per (slot, value head): T, P, scalars
   int32_t slices, members;  // scan: workgroups of a state, of a key head's group
@@ -88,10 +87,22 @@ struct Units {
 // Block (token tile, 32 columns) of T and P.
 __host__ __device__ constexpr int lower_block(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
 // Scalars of a (slot, value head): arrays of 64 floats.
-enum { kScIn = 0, kScQ = 1, kScOut = 2, kScMul = 3, kScEnd = 4 };
+enum { kScIn = 0, kScQ = 1, kScOut = 2, kScMul = 3, kScEnd = 4 };  // kScEnd: e^{G_end}, then whether to check
+// A column's largest value (see scan_kernel) that fits F16 through a chunk
+// whose rule is stable: no growing decay, 0 <= beta <= 2, |k| <= 2 and beta
+// |k|^2 <= 2. The step then does not stretch the state, |S| <= 16 max|S0| + 64
+// beta |k| max|v| in a column's 2-norm, and with both terms at most kColumnMost
+// the corrections, also times |k|, stay under 2 (kColumnMost + 2 kColumnMost) +
+// 2^8 < 2^16. Other chunks are checked value by value.
+constexpr float kColumnMost = 8192.0f, kColumnLeast = 64.0f, kColumnAim = 1024.0f;
 
-__device__ __forceinline__ int64_t slot_of(const PrefillArgs &a, int b, int first_token) {
-  return int64_t(first_token) * a.per_block / a.block + int64_t(a.slack) * b;
+// Row b's chunks start at slot first / 64 + b, and where they start anywhere in
+// a block at first / 64 + first / block + 3 b. That leaves n tokens room for
+// floor(n / 64) + 1 and floor(n / 64) + floor(n / block) + 3 chunks: cuts at
+// multiples of 64 inside blocks lie at least 64 tokens apart, so there are at
+// most floor((n - 1) / 64) + 1 of those and floor((n - 1) / block) + 1 at blocks.
+__host__ __device__ __forceinline__ int slot_of(bool align, int block, int b, int first_token) {
+  return align ? first_token / kChunk + int(unsigned(first_token) / unsigned(block)) + 3 * b : first_token / kChunk + b;
 }
 
 // Orders LDS across the workgroup without draining global loads in flight.
@@ -107,8 +118,12 @@ template <int PL>
 __device__ __forceinline__ void split2(float a, float b, uint32_t (&planes)[PL]) {
   const f16x2 hi = __builtin_convertvector(f32x2{a, b}, f16x2);
   planes[0] = __builtin_bit_cast(uint32_t, hi);
-  if constexpr (PL == 2)
-    planes[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - float(hi[0]), b - float(hi[1])}, f16x2));
+  if constexpr (PL == 2) {
+    float ra, rb;  // a - hi, b - hi: the mixed FMA reads the halves as they are
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(planes[0]), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(planes[0]), "v"(b));
+    planes[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
+  }
 }
 // Eight values as PL operand planes.
 template <int PL>
@@ -165,6 +180,13 @@ __device__ __forceinline__ float inverse_power(float x) {
   return e == 0xff || x == 0.0f ? 1.0f : __uint_as_float(uint32_t(254 - c) << 23);
 }
 
+// Whether a column's largest value needs no other scale, and the factor that
+// brings one past F16's reach back inside.
+__device__ __forceinline__ bool column_fits(float m) {
+  return m == 0.0f || !(m < kColumnLeast || m > kColumnMost) || m > 3e38f;
+}
+__device__ __forceinline__ float back_inside(float m) { return m > 32768.0f ? kColumnAim * inverse_power(m) : 1.0f; }
+
 // Inclusive sum over the wave's lanes in 64 bits.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add64(double x) {
@@ -213,6 +235,7 @@ __global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)
   constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, LD = kChunk + 4;
   constexpr int kLower = kChunk * LD * 4, kKeys = U::Q * kUnit;
   __shared__ __attribute__((aligned(16))) char lds[kLower > kKeys ? kLower : kKeys];
+  __shared__ float knorm[kChunk];  // |k|^2 as the rule sees it
   __shared__ float kmul[kChunk], qmul[kChunk];  // what a row of K and Q was divided by, times the L2 norm's factor
   float(*const Ls)[LD] = reinterpret_cast<float(*)[LD]>(lds);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -223,21 +246,23 @@ __global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)
   const int b = __builtin_amdgcn_readfirstlane(
       last_not_above(int(a.pages.rows), slot, [&](int i) {
         const int64_t at = load_index(a.pages.query_start_loc, i * a.pages.qsl_stride, a.pages.qsl_dtype);
-        return slot_of(a, i, clamp_token(at, a.pages.tokens));
+        return slot_of(a.align, a.block, i, clamp_token(at, a.pages.tokens));
       }));
   if (b < 0) return;
   const Row r = load_row(a.pages, b);
   if (r.n == 0 || !r.valid) return;
-  // The chunk's tokens.
-  const int64_t C = a.align ? r.C : 0;
-  const int64_t o = (C / a.block) * a.per_block + (C % a.block) / kChunk + (slot - slot_of(a, b, r.bos));
-  const int64_t blk = o / a.per_block;
-  int64_t p0 = blk * a.block + (o % a.per_block) * kChunk, p1 = p0 + kChunk;
-  p1 = p1 < (blk + 1) * a.block ? p1 : (blk + 1) * a.block;
-  p0 = p0 > C ? p0 : C;
-  p1 = p1 < C + r.n ? p1 : C + r.n;
+  // The chunk's tokens, from the row's first.
+  int p0 = (slot - slot_of(a.align, a.block, b, r.bos)) * kChunk, p1 = p0 + kChunk;
+  if (a.align) {
+    const int inside = int(r.C % a.block), o = inside / kChunk + p0 / kChunk;  // the row's first block starts `inside` before it
+    const int blk = int(unsigned(o) / unsigned(a.per_block));
+    p0 = blk * a.block + (o - blk * a.per_block) * kChunk - inside;
+    p1 = p0 + kChunk < (blk + 1) * a.block - inside ? p0 + kChunk : (blk + 1) * a.block - inside;
+    p0 = p0 > 0 ? p0 : 0;
+  }
+  p1 = p1 < r.n ? p1 : r.n;
   if (p0 >= p1) return;
-  const int t0 = r.bos + int(p0 - C), n = int(p1 - p0);
+  const int t0 = r.bos + p0, n = p1 - p0;
 
   // Gates, lane = token.
   const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
@@ -295,12 +320,12 @@ __global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)
     }
     // With x' = x div and div a power of two, x / sqrt(|x|^2 + 1e-6) =
     // x' / sqrt(|x'|^2 + 1e-6 div^2).
-    if (a.l2norm) {
-      ksq = sum_quarters(ksq);
-      qsq = sum_quarters(qsq);
-    }
+    ksq = sum_quarters(ksq);
+    qsq = sum_quarters(qsq);
     if (lq == 0) {
-      kmul[row] = a.l2norm ? 1.0f / sqrtf(ksq + 1e-6f * kdiv * kdiv) : 1.0f / kdiv;
+      const float km = a.l2norm ? 1.0f / sqrtf(ksq + 1e-6f * kdiv * kdiv) : 1.0f / kdiv;
+      kmul[row] = km;
+      knorm[row] = ksq * km * km;
       qmul[row] = a.l2norm ? 1.0f / sqrtf(qsq + 1e-6f * qdiv * qdiv) : 1.0f / qdiv;
     }
     __syncthreads();
@@ -363,7 +388,10 @@ __global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)
     sc[kScQ * 64 + lane] = e * (a.scale * qmul[lane] / mul);
     sc[kScOut * 64 + lane] = __builtin_amdgcn_exp2f(float(end - G)) * kmul[lane];
     sc[kScMul * 64 + lane] = mul;
-    sc[kScEnd * 64 + lane] = __builtin_amdgcn_exp2f(float(end));
+    const float k2 = knorm[lane];
+    const bool stable = g <= 0.0f && beta >= 0.0f && beta <= 2.0f && k2 <= 4.0f && beta * k2 <= 2.0f;
+    const bool check = __builtin_amdgcn_ballot_w64(!stable) != 0;
+    sc[kScEnd * 64 + lane] = lane == 0 ? __builtin_amdgcn_exp2f(float(end)) : check ? 1.0f : 0.0f;
   }
   // L and P, token rows 16w + 4 lq + i, columns 16j + lr.
   float Ght[4], Glt[4], bt[4], qt[4];
@@ -503,6 +531,13 @@ __device__ __forceinline__ void copy_units2(const char *src, uint32_t lane_at, u
       "s"(src), "s"(dst));
 }
 
+// A buffer of `bytes` in scalar registers, whatever made the two.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_buffer(const void *p, int bytes) {
+  const int64_t at = uniform64(int64_t(reinterpret_cast<uintptr_t>(p)));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(uintptr_t(at)), 0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
 // Whether two chunks' operands fit LDS; else waves read them from memory.
 constexpr bool scan_staged(int pl, int opl, int kp) { return 2 * (12 * (kp / 32) * pl + 14 + 6 * opl) <= 160; }
 
@@ -536,7 +571,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     }
     return;
   }
-  const int64_t slot = slot_of(a, b, r.bos);
+  const int64_t slot = slot_of(a.align, a.block, b, r.bos);
   const char *key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit);
   const char *value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit);
   const int64_t key_step = int64_t(a.H) * (U::KEY * kUnit), value_step = int64_t(a.HV) * (U::VALUE * kUnit);
@@ -558,7 +593,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     else return *reinterpret_cast<const u32x4 *>((u < U::KEY ? key_ws + u * kUnit : value_ws + (u - U::KEY) * kUnit) + lane_at);
   };
   const auto scalars = [&](int array, int tile) -> f32x4 {
-    const int at = array * 256 + (16 * tile + 4 * lq) * 4;
+    const int at = array * 256 + (tile < 0 ? 0 : (16 * tile + 4 * lq) * 4);  // tile < 0: the array's first four
     if constexpr (STAGED) return *reinterpret_cast<const f32x4 *>(lds + buffer + (U::KEY + U::SC) * kUnit + at);
     else return *reinterpret_cast<const f32x4 *>(value_ws + U::SC * kUnit + at);
   };
@@ -588,8 +623,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   const int out_col = column ? (v0 + lr) * ob + 4 * lq * out_bytes : kScanDead;
   uint32_t vv[4][4];
   const auto load_v = [&](int tokens) {
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(vp), 0,
-                                                      tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0, 0x00020000);
+    const auto rs = uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -655,9 +689,9 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     const int to = UNITS * kUnit - buffer;
     vp += int64_t(n) * v_bytes;
 
-    // Keep this column's values inside F16: with |k| near 1, |S0 k| is at most
-    // sqrt(K) <= 16 times S0's largest element, and where the rule is stable the
-    // corrections stay under 64 times v's largest plus that.
+    // Keep this column's values inside F16.
+    const f32x4 end4 = scalars(kScEnd, -1);
+    const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(end4[1])) != 0;
     {
       float ms = 0.0f, mv = 0.0f;
 #pragma unroll
@@ -665,8 +699,8 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) mv = largest(mv, f32x4{value(t, 0), value(t, 1), value(t, 2), value(t, 3)});
       const float m = max_quarters(fmaxf(16.0f * ms, 64.0f * sigma * mv));
-      const bool fits = m == 0.0f || !(m < 64.0f || m > 16384.0f) || m > 3e38f;
-      if (__builtin_amdgcn_ballot_w64(!fits) != 0) rescale(fits ? 1.0f : 2048.0f * inverse_power(m));
+      const bool fits = column_fits(m);
+      if (__builtin_amdgcn_ballot_w64(!fits) != 0) rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
     }
     // X = K S0^T and Q S0^T.
     f32x4 X[4], O[4];
@@ -706,17 +740,18 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     }
     // R = v - diag(e^G) X.
     f32x4 R[4];
-    float mr = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const f32x4 in = scalars(kScIn, t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) R[t][i] = fmaf(-in[i], X[t][i], sigma * value(t, i));
-      mr = largest(mr, R[t]);
     }
     load_v(n_next);
-    if (__builtin_amdgcn_ballot_w64(mr > 32768.0f) != 0) {
-      const float m = max_quarters(mr), f = m > 32768.0f ? 2048.0f * inverse_power(m) : 1.0f;
+    if (check) {
+      float m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) m = largest(m, R[t]);
+      const float f = back_inside(max_quarters(m));
       rescale(f);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -750,14 +785,13 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     }
     // d = diag(e^{G_end - G}) c.
     f32x4 d[4];
-    float mc = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      d[t] = c[t] * scalars(kScOut, t);
-      mc = largest(largest(mc, c[t]), d[t]);
-    }
-    if (__builtin_amdgcn_ballot_w64(mc > 32768.0f) != 0) {
-      const float m = max_quarters(mc), f = m > 32768.0f ? 2048.0f * inverse_power(m) : 1.0f;
+    for (int t = 0; t < 4; ++t) d[t] = c[t] * scalars(kScOut, t);
+    if (check) {
+      float m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) m = largest(largest(m, c[t]), d[t]);
+      const float f = back_inside(max_quarters(m));
       rescale(f);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -767,7 +801,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
       }
     }
     // S1 = e^{G_end} S0 + K^T d.
-    const float end = scalars(kScEnd, 0)[0];
+    const float end = end4[0];
 #pragma unroll
     for (int i = 0; i < NT; ++i) S[i] *= end;
 #pragma unroll
@@ -813,7 +847,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
     // that chunk's time.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     {
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(op, 0, (n - 1) * out_bytes + a.V * ob, 0x00020000);
+      const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 x = O[t] * (scalars(kScMul, t) * unscale);
@@ -841,6 +875,431 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   store_state(r.fin);
 }
 
+// ---------------------------------------------------------------------------
+// Scan, split: one workgroup of eight waves per (row, value head, 16 columns of
+// V). Four waves carry the chain from chunk to chunk (X = K S0^T, c = T (v - X),
+// S1), wave w with token rows 16w .. and key columns KP/4 * w ..; the other four
+// make the outputs beside them, from the planes of S0 and c that the chain
+// leaves in LDS anyway. For launches of too few columns to fill the chip, where
+// a row's chunks one after the other are all the time there is: a chunk is a
+// quarter of the instructions, for three exchanges through LDS. Operands go from
+// memory into the registers of the one wave that uses them, a chunk ahead: they
+// are refilled as soon as their product has taken them.
+// ---------------------------------------------------------------------------
+constexpr int kSplitThreads = 512;
+constexpr int split_waves(int pl, int kp) { return pl == 1 && kp <= 64 ? 4 : 2; }
+
+template <typename A, typename Out, int KP>
+__global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) void scan_split_kernel(
+    const PrefillArgs a) {
+  using U = Units<A, Out, KP>;
+  constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, KT = KP / 64, EB = int(sizeof(A)), ob = int(sizeof(Out));
+  // Operand planes in lane order, and per column the largest value of each
+  // chain wave.
+  __shared__ __attribute__((aligned(16))) char Sp[2][KS][kUnit], Rp[2][2][kUnit], Dp[2][2][kUnit], Cp[OPL][2][kUnit];
+  __shared__ __attribute__((aligned(16))) float top_s[16][4], top_r[16][4], top_c[16][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int lr = lane & 15, lq = lane >> 4;
+  const int wg = int(blockIdx.x), group = (wg / 8 / a.members) * 8 + wg % 8, member = wg / 8 % a.members;
+  if (group >= a.pages.rows * a.H) return;
+  const int b = group / a.H, h = group % a.H;
+  const int hv = h * a.ratio + member / a.slices, v0 = member % a.slices * 16;
+  const Row r = load_row(a.pages, b);
+  if (r.n == 0) return;
+  const bool column = v0 + lr < a.V;
+  if (!r.valid) {
+    for (int t = threadIdx.x >> 4; t < r.n; t += kSplitThreads / 16)
+      if (column)
+        static_cast<Out *>(a.out)[int64_t(r.bos + t) * a.out_ts + int64_t(hv) * a.V + v0 + lr] = from_f32<Out>(0.0f);
+    return;
+  }
+  const int64_t slot = slot_of(a.align, a.block, b, r.bos);
+  const int64_t key_step = int64_t(a.H) * (U::KEY * kUnit), value_step = int64_t(a.HV) * (U::VALUE * kUnit);
+  const char *const key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit);
+  const char *const value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit);
+  const int at4 = 16 * w + 4 * lq;
+  const bool low = w >= 2;  // T and P: columns 32 .. 63 are zero for the upper token rows
+  // Operand unit i of a wave-uniform run of units: the run's address advances in
+  // scalar registers, and every fourth unit has a lane offset of its own (an
+  // instruction's ends at 4 KB).
+  const uint32_t lane_at = lane * 16;
+  uint32_t unit_at[(KS * PL > 2 * KT * PL ? KS * PL : 2 * KT * PL) / 4 + 1];
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(unit_at) / 4; ++i) {
+    unit_at[i] = lane_at + i * 4 * kUnit;
+    asm("" : "+v"(unit_at[i]));
+  }
+  const auto operand = [&](const char *run, int i) {
+    return *reinterpret_cast<const u32x4 *>(run + unit_at[i >> 2] + (i & 3) * kUnit);
+  };
+  const char *sc = value_ws + U::SC * kUnit;
+  const uint32_t sc_at = at4 * 4;
+  const auto scalars = [&](int array) { return *reinterpret_cast<const f32x4 *>(sc + sc_at + array * 256); };
+  const auto shared = [&](const char *p) { return *reinterpret_cast<const u32x4 *>(p + lane_at); };
+  // The largest over the chain's waves of this lane's column.
+  const auto top = [&](const float (&t)[16][4]) { return largest(0.0f, *reinterpret_cast<const f32x4 *>(t[lr])); };
+
+  // Chunk lengths from position to position.
+  const auto length = [&](int at, int in) {
+    int n = kChunk - (in & (kChunk - 1));
+    n = n < a.block - in ? n : a.block - in;
+    return n < r.n - at ? n : r.n - at;
+  };
+  const auto after = [&](int in, int n) { return in + n == a.block ? 0 : in + n; };
+  int done = 0, inside = a.align ? int(r.C % a.block) : 0;
+  int n = length(0, inside);
+  float sigma = 1.0f, unscale = 1.0f;
+
+  if (wave >= 4) {
+    // ---- outputs ----
+    u32x4 qf[KS][PL], pf[2][OPL];
+    const int out_bytes = int(a.out_ts) * ob;
+    char *op = static_cast<char *>(a.out) + (r.bos * a.out_ts + int64_t(hv) * a.V) * ob;
+    int col[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * out_bytes + (v0 + lr) * ob : kScanDead;
+    const char *qp = key_ws + (U::Q + w * KS * PL) * kUnit;
+    const char *pp = value_ws + (U::P + lower_block(w, 0) * OPL) * kUnit;
+    const auto load_q = [&]() {
+#pragma unroll
+      for (int i = 0; i < KS * PL; ++i) qf[i / PL][i % PL] = operand(qp, i);
+    };
+    const auto load_p = [&]() {
+#pragma unroll
+      for (int p = 0; p < OPL; ++p) pf[0][p] = operand(pp, p);
+      if (low)
+#pragma unroll
+        for (int p = 0; p < OPL; ++p) pf[1][p] = operand(pp, OPL + p);
+    };
+    const auto load_check = [&]() { return *reinterpret_cast<const float *>(sc + kScEnd * 256 + 4); };
+    load_q();
+    f32x4 scale = scalars(kScQ);
+    float check_next = load_check();
+    load_p();
+    f32x4 mul = scalars(kScMul);
+    while (true) {
+      const int done_next = done + n, in_next = after(inside, n);
+      const bool more = done_next < r.n;
+      const int n_next = more ? length(done_next, in_next) : 0;
+      const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
+      qp += kstep;
+      pp += vstep;
+      sc += vstep;
+      const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(check_next)) != 0;
+      lds_barrier();  // S0
+      u32x4 sp[KS][OPL];
+      const auto read_s = [&]() {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int p = 0; p < OPL; ++p) sp[ks][p] = shared(Sp[p][ks]);
+      };
+      {
+        const float m = top(top_s);
+        read_s();
+        const bool fits = column_fits(m);
+        if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
+          unscale /= fits ? 1.0f : kColumnAim * inverse_power(m);
+          lds_barrier();
+          read_s();
+        }
+      }
+      f32x4 out = {0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) out = mfma_planes<PL, OPL>(qf[ks], sp[ks], out);
+      load_q();
+      out *= scale;
+      scale = scalars(kScQ);
+      check_next = load_check();
+      lds_barrier();  // R
+      if (check) {
+        const float f = back_inside(top(top_r));
+        out *= f;
+        unscale /= f;
+        lds_barrier();
+      }
+      lds_barrier();  // c
+      if (check) {
+        const float f = back_inside(top(top_c));
+        out *= f;
+        unscale /= f;
+        lds_barrier();
+      }
+      {
+        u32x4 cf[OPL];
+#pragma unroll
+        for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][0]);
+        out = mfma_planes<OPL, OPL>(pf[0], cf, out);
+      }
+      if (low) {
+        u32x4 cf[OPL];
+#pragma unroll
+        for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][1]);
+        out = mfma_planes<OPL, OPL>(pf[1], cf, out);
+      }
+      load_p();
+      const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
+      const f32x4 x = out * (mul * unscale);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, col[i], 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, col[i], 0, 0);
+      }
+      mul = scalars(kScMul);
+      if (!more) return;
+      op += n * out_bytes;
+      done = done_next;
+      inside = in_next;
+      n = n_next;
+    }
+  }
+
+  // ---- the chain ----
+  __builtin_amdgcn_s_setprio(2);
+  u32x4 kf[KS][PL], tf[2][2], kt[2][KT][PL];
+  uint32_t vv[4], v_next[4];  // of this chunk and the next
+  const int v_bytes = int(a.v_ts) * EB;
+  const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + r.bos * a.v_ts + int64_t(hv) * a.V);
+  int col[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * v_bytes + (v0 + lr) * EB : kScanDead;
+  const auto load_v = [&](int tokens, uint32_t (&to)[4]) {
+    const auto rs = uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (EB == 4) to[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, col[i], 0, 0);
+      else to[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, col[i], 0, 0);
+    }
+    vp += tokens * v_bytes;
+  };
+  const auto value = [&](uint32_t bits) {
+    if constexpr (EB == 4) return __uint_as_float(bits);
+    else return to_f32(__builtin_bit_cast(A, uint16_t(bits)));
+  };
+  const char *kp = key_ws + w * KS * PL * kUnit, *ktp = key_ws + (U::KT + w * KT * 2 * PL) * kUnit;
+  const char *tp = value_ws + lower_block(w, 0) * 2 * kUnit;
+  const auto load_k = [&]() {
+#pragma unroll
+    for (int i = 0; i < KS * PL; ++i) kf[i / PL][i % PL] = operand(kp, i);
+  };
+  const auto load_t = [&]() {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) tf[0][p] = operand(tp, p);
+    if (low)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) tf[1][p] = operand(tp, 2 + p);
+  };
+  const auto load_kt = [&]() {
+#pragma unroll
+    for (int i = 0; i < KT * 2 * PL; ++i) kt[i / PL % 2][i / (2 * PL)][i % PL] = operand(ktp, i);
+  };
+  const auto load_end = [&]() { return *reinterpret_cast<const f32x2 *>(sc + kScEnd * 256); };
+
+  const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
+    return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * (w * KT + i) + 4 * lq;
+  };
+  f32x4 S[KT];
+  const auto store_state = [&](int64_t page) {
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+      if (column && 16 * (w * KT + i) + 4 * lq < a.K) {
+        const int64_t at = state_at(page, i);
+        const f32x4 x = S[i] * unscale;
+        if (a.state_dt == GDN_DT_F32) {
+          *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
+        } else if (a.state_dt == GDN_DT_BF16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+        }
+      }
+  };
+  const auto rescale = [&](float f) {
+#pragma unroll
+    for (int i = 0; i < KT; ++i) S[i] *= f;
+    sigma *= f;
+    unscale /= f;
+  };
+  // Planes of the wave's S tiles, in operand order: tile i is half i % 2 of
+  // columns 32 (i / 2) ...
+  const auto publish_s = [&]() {
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      const int tile = w * KT + i;
+      uint32_t lo[2], hi[2];
+      split2<2>(S[i][0], S[i][1], lo);
+      split2<2>(S[i][2], S[i][3], hi);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        *reinterpret_cast<u32x2 *>(&Sp[p][tile >> 1][lane_at + (tile & 1) * 8]) = u32x2{lo[p], hi[p]};
+    }
+  };
+  const uint32_t row_at = (w >> 1) * kUnit + lane_at + (w & 1) * 8;
+  const auto publish_rows = [&](const f32x4 &x, auto planes, char *to) {  // to: [planes][2][kUnit]
+    constexpr int N = decltype(planes)::value;
+    uint32_t lo[N], hi[N];
+    split2<N>(x[0], x[1], lo);
+    split2<N>(x[2], x[3], hi);
+#pragma unroll
+    for (int p = 0; p < N; ++p) *reinterpret_cast<u32x2 *>(to + p * 2 * kUnit + row_at) = u32x2{lo[p], hi[p]};
+  };
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, OPL> out_pl{};
+  const auto publish_top = [&](float m, float (&t)[16][4]) {
+    m = max_quarters(m);
+    if (lq == 0) t[lr][w] = m;
+  };
+  const auto top_state = [&](const uint32_t (&v)[4]) {
+    float ms = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KT; ++i) ms = largest(ms, S[i]);
+    const float mv = largest(0.0f, f32x4{value(v[0]), value(v[1]), value(v[2]), value(v[3])});
+    publish_top(largest(0.0f, f32x4{16.0f * ms, 64.0f * sigma * mv, 0.0f, 0.0f}), top_s);
+  };
+
+  load_k();
+  f32x4 in_scale = scalars(kScIn);
+  load_v(n, vv);
+  // The next two chunks' tokens: their lengths are needed as their loads start.
+  int in_1 = after(inside, n), n_1 = n < r.n ? length(n, in_1) : 0;
+  load_v(n_1, v_next);
+#pragma unroll
+  for (int i = 0; i < KT; ++i) {
+    S[i] = f32x4{0, 0, 0, 0};
+    if (!r.fresh && column && 16 * (w * KT + i) + 4 * lq < a.K)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
+  }
+  load_t();
+  f32x4 out_decay = scalars(kScOut);
+  load_kt();
+  f32x2 end_check = load_end();
+  top_state(vv);
+  publish_s();
+
+  while (true) {
+    const int done_next = done + n, done_2 = done_next + n_1;
+    const bool more = done_next < r.n;
+    const int in_2 = after(in_1, n_1), n_2 = done_2 < r.n ? length(done_2, in_2) : 0;
+    const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
+    kp += kstep;
+    ktp += kstep;
+    tp += vstep;
+    sc += vstep;
+    const float end = end_check[0];
+    const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(end_check[1])) != 0;
+    // First of the next chunk's loads, because it is the first to be waited for.
+    end_check = load_end();
+    lds_barrier();
+    // Planes are read before the columns' sizes are looked at, and again where
+    // those call for it.
+    u32x4 sp[KS][2];
+    const auto read_s = [&]() {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) sp[ks][p] = shared(Sp[p][ks]);
+    };
+    {
+      const float m = top(top_s);
+      read_s();
+      const bool fits = column_fits(m);
+      if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
+        rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
+        publish_s();
+        lds_barrier();
+        read_s();
+      }
+    }
+    // X = K S0^T.
+    f32x4 X[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      X[0] = mfma(kf[ks][0], sp[ks][0], X[0]);
+      X[1] = mfma(kf[ks][0], sp[ks][1], X[1]);
+      if constexpr (PL == 2) X[1] = mfma(kf[ks][1], sp[ks][0], X[1]);
+    }
+    load_k();
+    // R = v - diag(e^G) X.
+    f32x4 R;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) R[i] = fmaf(-in_scale[i], X[0][i] + X[1][i], sigma * value(vv[i]));
+    publish_rows(R, two, &Rp[0][0][0]);
+    if (check) publish_top(largest(0.0f, R), top_r);
+    in_scale = scalars(kScIn);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vv[i] = v_next[i];
+    load_v(n_2, v_next);
+    lds_barrier();
+    if (check) {
+      const float f = back_inside(top(top_r));
+      R *= f;
+      rescale(f);
+      publish_rows(R, two, &Rp[0][0][0]);
+      lds_barrier();
+    }
+    // c = T R, d = diag(e^{G_end - G}) c.
+    f32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    {
+      const u32x4 hi = shared(Rp[0][0]), lo = shared(Rp[1][0]);
+      c[0] = mfma(tf[0][0], hi, c[0]);
+      c[1] = mfma(tf[0][1], hi, c[1]);
+      c[1] = mfma(tf[0][0], lo, c[1]);
+    }
+    if (low) {
+      const u32x4 hi = shared(Rp[0][1]), lo = shared(Rp[1][1]);
+      c[0] = mfma(tf[1][0], hi, c[0]);
+      c[1] = mfma(tf[1][1], hi, c[1]);
+      c[1] = mfma(tf[1][0], lo, c[1]);
+    }
+    load_t();
+    c[0] += c[1];
+    f32x4 d = c[0] * out_decay;
+    publish_rows(d, two, &Dp[0][0][0]);
+    publish_rows(c[0], out_pl, &Cp[0][0][0]);
+    if (check) publish_top(largest(largest(0.0f, c[0]), d), top_c);
+    out_decay = scalars(kScOut);
+    lds_barrier();
+    if (check) {
+      const float f = back_inside(top(top_c));
+      rescale(f);
+      publish_rows(d * f, two, &Dp[0][0][0]);
+      publish_rows(c[0] * f, out_pl, &Cp[0][0][0]);
+      lds_barrier();
+    }
+    // S1 = e^{G_end} S0 + K^T d.
+#pragma unroll
+    for (int i = 0; i < KT; ++i) S[i] *= end;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const u32x4 hi = shared(Dp[0][ks]), lo = shared(Dp[1][ks]);
+#pragma unroll
+      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], hi, S[i]);
+#pragma unroll
+      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], lo, S[i]);
+      if constexpr (PL == 2)
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][1], hi, S[i]);
+    }
+    load_kt();
+    if (!more) break;
+    publish_s();
+    top_state(vv);
+    if (a.align && in_1 == 0) {
+      const int64_t page = boundary_page(a.pages, r, r.C + done_next);
+      if (page != 0) store_state(page);
+    }
+    done = done_next;
+    n = n_1;
+    in_1 = in_2;
+    n_1 = n_2;
+  }
+  store_state(r.fin);
+}
+
 template <typename A, typename Out, int KP, int NW>
 static void launch_scan(unsigned grid, hipStream_t s, const PrefillArgs &a) {
   using U = Units<A, Out, KP>;
@@ -850,6 +1309,10 @@ static void launch_scan(unsigned grid, hipStream_t s, const PrefillArgs &a) {
 template <typename A, typename Out, int KP>
 static void launch_prefill_dims(int nw, unsigned scan_grid, hipStream_t s, const PrefillArgs &a) {
   hipLaunchKernelGGL((prepare_kernel<A, Out, KP>), dim3(unsigned(a.slots) * unsigned(a.HV)), dim3(kPrepareThreads), 0, s, a);
+  if (nw == 0) {
+    hipLaunchKernelGGL((scan_split_kernel<A, Out, KP>), dim3(scan_grid), dim3(kSplitThreads), 0, s, a);
+    return;
+  }
   if constexpr (scan_staged(key_planes<A>(), out_planes<Out>(), KP)) {
     if (nw == 1) return launch_scan<A, Out, KP, 1>(scan_grid, s, a);
     if (nw == 2) return launch_scan<A, Out, KP, 2>(scan_grid, s, a);
