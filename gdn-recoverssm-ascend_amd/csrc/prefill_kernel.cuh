@@ -205,11 +205,14 @@ __device__ __forceinline__ double wave_prefix(double x) {
 }
 
 // ---------------------------------------------------------------------------
-// Prepare: one workgroup of four waves per (slot, value head); the first of a
-// key head's value heads also packs K, Q and K^T. Wave w holds token rows 16w
-// .. 16w + 15 of K K^T and Q K^T.
+// Prepare: one workgroup per (slot, key head): the planes of K, Q and K^T, the
+// products K K^T and Q K^T, and T, P and the scalars of each of its value heads.
+// A team of four waves takes a value head, wave w token rows 16w .. 16w + 15;
+// with two teams one loads K and the other Q, and each takes every second value
+// head. Bound by vector instructions: most of a wave's go into converting K and
+// Q and into L and P.
 // ---------------------------------------------------------------------------
-constexpr int kPrepareThreads = 256;
+constexpr int prepare_waves(int pl, int kp) { return pl == 1 && kp <= 128 ? 4 : pl == 1 || kp <= 128 ? 2 : 1; }
 
 // The lane's eight columns of a token row in operand order.
 template <typename A>
@@ -227,22 +230,21 @@ __device__ __forceinline__ void load_row8(const A *row, bool live, int k0, int K
   }
 }
 
-constexpr int prepare_waves(int pl, int kp) { return pl == 1 && kp <= 128 ? 4 : pl == 1 || kp <= 128 ? 2 : 1; }
-
-template <typename A, typename Out, int KP>
-__global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)) void prepare_kernel(const PrefillArgs a) {
+template <typename A, typename Out, int KP, int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) void prepare_kernel(const PrefillArgs a) {
   using U = Units<A, Out, KP>;
   constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, LD = kChunk + 4;
-  constexpr int kLower = kChunk * LD * 4, kKeys = U::Q * kUnit;
-  __shared__ __attribute__((aligned(16))) char lds[kLower > kKeys ? kLower : kKeys];
-  __shared__ float knorm[kChunk];  // |k|^2 as the rule sees it
+  // Planes of K and Q, then, in their place, a matrix of a value head per team.
+  constexpr int kSide = U::Q * kUnit, kMatrix = kChunk * LD * 4;
+  constexpr int kLds = 2 * kSide > TEAMS * kMatrix ? 2 * kSide : TEAMS * kMatrix;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
   __shared__ float kmul[kChunk], qmul[kChunk];  // what a row of K and Q was divided by, times the L2 norm's factor
-  float(*const Ls)[LD] = reinterpret_cast<float(*)[LD]>(lds);
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float knorm[kChunk];               // |k|^2 as the rule sees it
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = wave & 3, team = TEAMS == 1 ? 0 : wave >> 2;
   const int lr = lane & 15, lq = lane >> 4;
-  const int slot = int(blockIdx.x / unsigned(a.HV)), hv = int(blockIdx.x % unsigned(a.HV));
-  const int h = hv / a.ratio;
-  const bool packs = hv % a.ratio == 0;
+  float(*const Ls)[LD] = reinterpret_cast<float(*)[LD]>(lds + team * kMatrix);
+  const int slot = int(blockIdx.x / unsigned(a.H)), h = int(blockIdx.x % unsigned(a.H));
   const int b = __builtin_amdgcn_readfirstlane(
       last_not_above(int(a.pages.rows), slot, [&](int i) {
         const int64_t at = load_index(a.pages.query_start_loc, i * a.pages.qsl_stride, a.pages.qsl_dtype);
@@ -264,236 +266,275 @@ __global__ __launch_bounds__(kPrepareThreads, prepare_waves(key_planes<A>(), KP)
   if (p0 >= p1) return;
   const int t0 = r.bos + p0, n = p1 - p0;
 
-  // Gates, lane = token.
-  const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
-  float g = 0.0f, beta = 0.0f;
-  if (lane < n) {
-    g = load_as_f32(a.g, int64_t(t0 + lane) * a.g_ts + hv, a.g_dt);
-    beta = load_as_f32(a.beta, int64_t(t0 + lane) * a.beta_ts + hv, a.beta_dt);
-  }
-
-  // K and Q rows of this wave, scaled by powers of two.
-  f32x4 kk[4], qk[4];
+  // Rows of K or Q, scaled by powers of two, as planes in LDS and the workspace.
   const int row = 16 * w + lr;
   char *const key_ws = a.ws + (int64_t(slot) * a.H + h) * (U::KEY * kUnit);
-  {
-    const A *const kp = static_cast<const A *>(a.k) + int64_t(t0 + row) * a.k_ts + int64_t(h) * a.K;
-    const A *const qp = static_cast<const A *>(a.q) + int64_t(t0 + row) * a.q_ts + int64_t(h) * a.K;
-    f32x4 kx[KS][2], qx[KS][2];
+  const auto side = [&](bool is_q) {
+    const A *const src = static_cast<const A *>(is_q ? a.q : a.k) + int64_t(t0 + row) * (is_q ? a.q_ts : a.k_ts) + h * a.K;
+    f32x4 x[KS][2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) load_row8(src, row < n, 32 * ks + 4 * lq, a.K, x[ks]);
+    float top = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) top = largest(largest(top, x[ks][0]), x[ks][1]);
+    const float div = inverse_power(max_quarters(top));
+    char *const to = key_ws + (is_q ? U::Q * kUnit : 0);
+    char *const near = lds + (is_q ? kSide : 0);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      load_row8(kp, row < n, 32 * ks + 4 * lq, a.K, kx[ks]);
-      load_row8(qp, row < n, 32 * ks + 4 * lq, a.K, qx[ks]);
-    }
-    float kmax = 0.0f, qmax = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        kmax = fmaxf(kmax, fabsf(kx[ks][i >> 2][i & 3]));
-        qmax = fmaxf(qmax, fabsf(qx[ks][i >> 2][i & 3]));
-      }
-    const float kdiv = inverse_power(max_quarters(kmax)), qdiv = inverse_power(max_quarters(qmax));
-    float ksq = 0.0f, qsq = 0.0f;
-    u32x4 kf[KS][PL], qf[KS][PL];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float kv = kx[ks][i >> 2][i & 3] * kdiv, qv = qx[ks][i >> 2][i & 3] * qdiv;
-        kx[ks][i >> 2][i & 3] = kv;
-        qx[ks][i >> 2][i & 3] = qv;
-        ksq = fmaf(kv, kv, ksq);
-        qsq = fmaf(qv, qv, qsq);
-      }
-      split8<PL>(kx[ks][0], kx[ks][1], kf[ks]);
-      split8<PL>(qx[ks][0], qx[ks][1], qf[ks]);
+      x[ks][0] *= div;
+      x[ks][1] *= div;
+      u32x4 f[PL];
+      split8<PL>(x[ks][0], x[ks][1], f);
 #pragma unroll
       for (int p = 0; p < PL; ++p) {
         const int at = ((w * KS + ks) * PL + p) * kUnit + lane * 16;
-        *reinterpret_cast<u32x4 *>(lds + at) = kf[ks][p];
-        if (packs) {
-          *reinterpret_cast<u32x4 *>(key_ws + at) = kf[ks][p];
-          *reinterpret_cast<u32x4 *>(key_ws + U::Q * kUnit + at) = qf[ks][p];
-        }
+        *reinterpret_cast<u32x4 *>(near + at) = f[p];
+        *reinterpret_cast<u32x4 *>(to + at) = f[p];
       }
     }
     // With x' = x div and div a power of two, x / sqrt(|x|^2 + 1e-6) =
     // x' / sqrt(|x'|^2 + 1e-6 div^2).
-    ksq = sum_quarters(ksq);
-    qsq = sum_quarters(qsq);
-    if (lq == 0) {
-      const float km = a.l2norm ? 1.0f / sqrtf(ksq + 1e-6f * kdiv * kdiv) : 1.0f / kdiv;
-      kmul[row] = km;
-      knorm[row] = ksq * km * km;
-      qmul[row] = a.l2norm ? 1.0f / sqrtf(qsq + 1e-6f * qdiv * qdiv) : 1.0f / qdiv;
+    float sq = 0.0f;
+    if (a.l2norm || !is_q) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(x[ks][i >> 2][i & 3], x[ks][i >> 2][i & 3], sq);
+      sq = sum_quarters(sq);
     }
-    __syncthreads();
+    if (lq == 0) {
+      const float mul = a.l2norm ? 1.0f / sqrtf(sq + 1e-6f * div * div) : 1.0f / div;
+      (is_q ? qmul : kmul)[row] = mul;
+      if (!is_q) knorm[row] = sq * mul * mul;
+    }
+  };
+  if (TEAMS == 1 || team == 0) side(false);
+  if (TEAMS == 1 || team == 1) side(true);
+  __syncthreads();
+  const auto plane = [&](int base, int tile, int ks, int p) {
+    return *reinterpret_cast<const u32x4 *>(lds + base + ((tile * KS + ks) * PL + p) * kUnit + lane * 16);
+  };
+  f32x4 kk[4], qk[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) kk[j] = qk[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    u32x4 kf[PL], qf[PL];
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      kf[p] = plane(0, w, ks, p);
+      qf[p] = plane(kSide, w, ks, p);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      kk[j] = f32x4{0, 0, 0, 0};
-      qk[j] = f32x4{0, 0, 0, 0};
-      if (j <= w) {
+      if (j > w) break;
+      u32x4 kb[PL];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          u32x4 kb[PL];
-#pragma unroll
-          for (int p = 0; p < PL; ++p)
-            kb[p] = *reinterpret_cast<const u32x4 *>(lds + ((j * KS + ks) * PL + p) * kUnit + lane * 16);
-          kk[j] = mfma_planes<PL, PL>(kf[ks], kb, kk[j]);
-          qk[j] = mfma_planes<PL, PL>(qf[ks], kb, qk[j]);
-        }
-      }
+      for (int p = 0; p < PL; ++p) kb[p] = plane(0, j, ks, p);
+      kk[j] = mfma_planes<PL, PL>(kf, kb, kk[j]);
+      qk[j] = mfma_planes<PL, PL>(qf, kb, qk[j]);
     }
   }
   // K^T: column 16 i + lr of K, tokens in operand order.
-  if (packs) {
-    for (int f = w; f < KP / 8; f += 4) {
-      const int i = f >> 1, ts = f & 1;
-      // Element (token, column) lies in K's planes at token tile, columns / 32,
-      // lane (column % 16 / 4) * 16 + token % 16, half column % 32 / 16, place
-      // column % 4.
-      const int base = ((i >> 1) * PL) * kUnit + ((lr >> 2) * 16) * 16 + (i & 1) * 8 + (lr & 3) * 2;
+  for (int f = wave; f < KP / 8; f += 4 * TEAMS) {
+    const int i = f >> 1, ts = f & 1;
+    // Element (token, column) lies in K's planes at token tile, columns / 32,
+    // lane (column % 16 / 4) * 16 + token % 16, half column % 32 / 16, place
+    // column % 4.
+    const int base = ((i >> 1) * PL) * kUnit + ((lr >> 2) * 16) * 16 + (i & 1) * 8 + (lr & 3) * 2;
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
-        u32x4 kt;
+    for (int p = 0; p < PL; ++p) {
+      u32x4 kt;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int tile = 2 * ts + (e >> 2), t = 4 * lq + (e & 3);
-          const char *at = lds + base + (tile * KS * PL + p) * kUnit + t * 16;
-          kt[e / 2] = uint32_t(*reinterpret_cast<const uint16_t *>(at)) |
-                      uint32_t(*reinterpret_cast<const uint16_t *>(at + 16)) << 16;
-        }
-        *reinterpret_cast<u32x4 *>(key_ws + (U::KT + f * PL + p) * kUnit + lane * 16) = kt;
+      for (int e = 0; e < 8; e += 2) {
+        const int tile = 2 * ts + (e >> 2), t = 4 * lq + (e & 3);
+        const char *at = lds + base + (tile * KS * PL + p) * kUnit + t * 16;
+        kt[e / 2] = uint32_t(*reinterpret_cast<const uint16_t *>(at)) |
+                    uint32_t(*reinterpret_cast<const uint16_t *>(at + 16)) << 16;
       }
+      *reinterpret_cast<u32x4 *>(key_ws + (U::KT + f * PL + p) * kUnit + lane * 16) = kt;
     }
   }
   __syncthreads();
 
-  // The cumulative log decay (base 2), summed in 64 bits and kept as two
-  // floats, so that differences keep FP32 precision however far the sum goes.
-  g = log_decay(gates, g);
-  g = lane < n ? (g < kMinLogDecay ? kMinLogDecay : g) : 0.0f;
-  beta = lane < n ? beta_of(gates, beta) : 0.0f;
-  const double G = wave_prefix(double(g) * 1.4426950408889634);
-  const float Gh = float(G), Gl = float(G - double(Gh));
-  char *const value_ws = a.ws_value + (int64_t(slot) * a.HV + hv) * (U::VALUE * kUnit);
-  if (w == 0) {
-    const double end = __shfl(G, 63);
-    float *sc = reinterpret_cast<float *>(value_ws + U::SC * kUnit);
-    const float e = __builtin_amdgcn_exp2f(Gh + Gl);
-    // The outputs' own scale: a power of two near Q's row, so that P fits F16.
-    const float mul = 1.0f / inverse_power(qmul[lane] * a.scale);
-    sc[kScIn * 64 + lane] = e * kmul[lane];
-    sc[kScQ * 64 + lane] = e * (a.scale * qmul[lane] / mul);
-    sc[kScOut * 64 + lane] = __builtin_amdgcn_exp2f(float(end - G)) * kmul[lane];
-    sc[kScMul * 64 + lane] = mul;
-    const float k2 = knorm[lane];
-    const bool stable = g <= 0.0f && beta >= 0.0f && beta <= 2.0f && k2 <= 4.0f && beta * k2 <= 2.0f;
-    const bool check = __builtin_amdgcn_ballot_w64(!stable) != 0;
-    sc[kScEnd * 64 + lane] = lane == 0 ? __builtin_amdgcn_exp2f(float(end)) : check ? 1.0f : 0.0f;
-  }
-  // L and P, token rows 16w + 4 lq + i, columns 16j + lr.
-  float Ght[4], Glt[4], bt[4], qt[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 16 * w + 4 * lq + i;
-    Ght[i] = __shfl(Gh, t);
-    Glt[i] = __shfl(Gl, t);
-    bt[i] = __shfl(beta, t) * kmul[t];
-    const float qs = qmul[t] * a.scale;
-    qt[i] = qs * inverse_power(qs);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int s = 16 * j + lr;
-    const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s), km = kmul[s];
+  for (int m0 = 0; m0 < a.ratio; m0 += TEAMS) {
+    // A team without a value head left still meets the barriers.
+    const bool works = m0 + team < a.ratio;
+    const int hv = h * a.ratio + (works ? m0 + team : m0);
+    char *const value_ws = a.ws_value + (int64_t(slot) * a.HV + hv) * (U::VALUE * kUnit);
+    // Gates, lane = token.
+    const GateParams gates = load_gates(a.a_log, a.dt_bias, a.gating, a.gated != 0, hv);
+    float g = 0.0f, beta = 0.0f;
+    if (lane < n) {
+      g = log_decay(gates, load_as_f32(a.g, int64_t(t0 + lane) * a.g_ts + hv, a.g_dt));
+      beta = beta_of(gates, load_as_f32(a.beta, int64_t(t0 + lane) * a.beta_ts + hv, a.beta_dt));
+      g = g < kMinLogDecay ? kMinLogDecay : g;
+    }
+    // The cumulative log decay (base 2), summed in 64 bits and kept as two
+    // floats, so that differences keep FP32 precision however far the sum goes.
+    const double G = wave_prefix(double(g) * 1.4426950408889634);
+    const float Gh = float(G), Gl = float(G - double(Gh));
+    const float qscale = qmul[lane] * a.scale, qdown = inverse_power(qscale);
+    const float bk = beta * kmul[lane], qn = qscale * qdown, km = kmul[lane];
+    if (w == 0 && works) {
+      const double end = __shfl(G, 63);
+      float *sc = reinterpret_cast<float *>(value_ws + U::SC * kUnit);
+      const float e = __builtin_amdgcn_exp2f(Gh + Gl);
+      sc[kScIn * 64 + lane] = e * km;
+      // The outputs' own scale: a power of two near Q's row, so that P fits F16.
+      sc[kScQ * 64 + lane] = e * qn;
+      sc[kScOut * 64 + lane] = __builtin_amdgcn_exp2f(float(end - G)) * km;
+      sc[kScMul * 64 + lane] = 1.0f / qdown;
+      const float k2 = knorm[lane];
+      const bool stable = g <= 0.0f && beta >= 0.0f && beta <= 2.0f && k2 <= 4.0f && beta * k2 <= 2.0f;
+      const bool check = __builtin_amdgcn_ballot_w64(!stable) != 0;
+      sc[kScEnd * 64 + lane] = lane == 0 ? __builtin_amdgcn_exp2f(float(end)) : check ? 1.0f : 0.0f;
+    }
+    // L and P, token rows 16w + 4 lq + i, columns 16j + lr. Off the diagonal
+    // e^{G_t - G_s} is e^{G_t - G_r} e^{G_r - G_s} with r the block's last
+    // column: five exponentials a lane for four elements' sixteen.
+    float Ght[4], Glt[4], bt[4], qt[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 16 * w + 4 * lq + i;
-      const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghs) + (Glt[i] - Gls)) * km;
-      Ls[t][s] = s < t ? bt[i] * d * kk[j][i] : 0.0f;
-      qk[j][i] = s <= t ? qt[i] * d * qk[j][i] : 0.0f;
+      Ght[i] = __shfl(Gh, t);
+      Glt[i] = __shfl(Gl, t);
+      bt[i] = __shfl(bk, t);
+      qt[i] = __shfl(qn, t);
     }
-  }
-  wave_fence();
-  // The diagonal block's inverse, a column a lane: x_i = [i = c] - sum_m L_im x_m.
-  f32x4 T[4];  // T[d]: block (w + d, w)
-  {
-    float x[16];
+    f32x4 P[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float s = i == lr ? 1.0f : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      const int s = 16 * j + lr;
+      P[j] = f32x4{0, 0, 0, 0};
+      f32x4 L = {0, 0, 0, 0};
+      if (j < w) {
+        const float Ghr = __shfl(Gh, 16 * j + 15), Glr = __shfl(Gl, 16 * j + 15);
+        const float col = __builtin_amdgcn_exp2f((Ghr - __shfl(Gh, s)) + (Glr - __shfl(Gl, s))) * __shfl(km, s);
 #pragma unroll
-      for (int c = 0; c < i; ++c) s = fmaf(-Ls[16 * w + i][16 * w + c], x[c], s);
-      x[i] = s;
-    }
+        for (int i = 0; i < 4; ++i) {
+          const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghr) + (Glt[i] - Glr)) * col;
+          L[i] = bt[i] * d * kk[j][i];
+          P[j][i] = qt[i] * d * qk[j][i];
+        }
+      } else if (j == w) {
+        const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s), kms = __shfl(km, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) T[0][i] = lq == 0 ? x[i] : lq == 1 ? x[4 + i] : lq == 2 ? x[8 + i] : x[12 + i];
-  }
-  wave_fence();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * w + lr] = T[0][i];
-  __syncthreads();
-  // Block column w downwards: T_iw = -T_ii sum_{m = w}^{i - 1} L_im T_mw. Step i
-  // of the FP32 instruction takes columns 4 lq + i, which is where the
-  // accumulator of the block before holds its rows: no value moves. Two
-  // accumulators, because a product waits for the one before it on its own.
-#pragma unroll
-  for (int d = 1; d < 4; ++d) {
-    const int i = w + d;
-    T[d] = f32x4{0, 0, 0, 0};
-    if (i < 4) {
-      f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-      for (int e = 0; e < d; ++e) {
-        const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * (w + e) + 4 * lq]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          acc[k & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[k], T[e][k], acc[k & 1], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const int t = 4 * lq + i;
+          const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghs) + (Glt[i] - Gls)) * kms;
+          L[i] = lr < t ? bt[i] * d * kk[j][i] : 0.0f;
+          P[j][i] = lr <= t ? qt[i] * d * qk[j][i] : 0.0f;
+        }
       }
-      const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * i + 4 * lq]);
-      acc[0] += acc[1];
-      acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][s] = L[i];
+    }
+    wave_fence();
+    // The diagonal block's inverse. First its two 8 x 8 diagonal blocks, a column
+    // a lane, x_i = [i = c] - sum_m L_im x_m; then with D their inverses and O
+    // the block below, D - D O D.
+    f32x4 T[4];  // T[d]: block (w + d, w)
+    {
+      const int half = lr >> 3, c0 = lr & 7, at = 16 * w + 8 * half;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float s = i == c0 ? 1.0f : 0.0f;
+#pragma unroll
+        for (int c = 0; c < i; ++c) s = fmaf(-Ls[at + i][at + c], x[c], s);
+        x[i] = s;
+      }
+      f32x4 D;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) D[i] = (lq >> 1) == half ? ((lq & 1) ? x[4 + i] : x[i]) : 0.0f;
+      f32x4 below = *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][16 * w + 4 * lq]);
+      below = lr >= 8 && lq < 2 ? below : f32x4{0, 0, 0, 0};
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * w + lr] = D[i];
+      wave_fence();
+      const f32x4 rows = *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][16 * w + 4 * lq]);
+      // Step k of the FP32 instruction takes columns 4 lq + k, which is where an
+      // accumulator holds its rows: no value moves.
+      f32x4 od[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) od[k & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(below[k], D[k], od[k & 1], 0, 0, 0);
+      od[0] += od[1];
+      od[1] = f32x4{0, 0, 0, 0};
+      T[0] = D;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        f32x4 &to = k & 1 ? acc[1] : T[d];
-        to = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[k], acc[0][k], to, 0, 0, 0);
+        f32x4 &to = k & 1 ? od[1] : T[0];
+        to = __builtin_amdgcn_mfma_f32_16x16x4f32(-rows[k], od[0][k], to, 0, 0, 0);
       }
-      T[d] += acc[1];
+      T[0] += od[1];
     }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * w + lr] = T[0][i];
+    __syncthreads();
+    // Block column w downwards: T_iw = -T_ii sum_{m = w}^{i - 1} L_im T_mw. Two
+    // accumulators, because a product waits for the one before it on its own.
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      const int i = w + d;
+      T[d] = f32x4{0, 0, 0, 0};
+      if (i < 4) {
+        f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int e = 0; e < d; ++e) {
+          const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * (w + e) + 4 * lq]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            acc[k & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(l[k], T[e][k], acc[k & 1], 0, 0, 0);
+        }
+        const f32x4 l = *reinterpret_cast<const f32x4 *>(&Ls[16 * i + lr][16 * i + 4 * lq]);
+        acc[0] += acc[1];
+        acc[1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f32x4 &to = k & 1 ? acc[1] : T[d];
+          to = __builtin_amdgcn_mfma_f32_16x16x4f32(-l[k], acc[0][k], to, 0, 0, 0);
+        }
+        T[d] += acc[1];
+      }
+    }
+    __syncthreads();
+    const float bs = __shfl(beta, 16 * w + lr);
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      if (w + d < 4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Ls[16 * (w + d) + 4 * lq + i][16 * w + lr] = T[d][i] * bs;
+    __syncthreads();
+    // Rows of T, then of P, as operands.
+    const auto rows_out = [&](auto planes, int unit) {
+      constexpr int N = decltype(planes)::value;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks == 1 && w < 2) continue;
+        u32x4 f[N];
+        split8<N>(*reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 4 * lq]),
+                  *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 16 + 4 * lq]), f);
+        if (works)
+#pragma unroll
+          for (int p = 0; p < N; ++p)
+            *reinterpret_cast<u32x4 *>(value_ws + (unit + lower_block(w, ks) * N + p) * kUnit + lane * 16) = f[p];
+      }
+    };
+    rows_out(std::integral_constant<int, 2>{}, 0);
+    wave_fence();
+    // A wave's rows of T are its own from here: P takes their place.
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * j + lr] = P[j][i];
+    wave_fence();
+    rows_out(std::integral_constant<int, OPL>{}, U::P);
+    wave_fence();
   }
-  __syncthreads();
-  const float bs = __shfl(beta, 16 * w + lr);
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-    if (w + d < 4)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Ls[16 * (w + d) + 4 * lq + i][16 * w + lr] = T[d][i] * bs;
-  __syncthreads();
-  // Rows of T, then of P, as operands.
-  const auto rows_out = [&](auto planes, int unit) {
-    constexpr int N = decltype(planes)::value;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      if (ks == 1 && w < 2) continue;
-      u32x4 f[N];
-      split8<N>(*reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 4 * lq]),
-                *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][32 * ks + 16 + 4 * lq]), f);
-#pragma unroll
-      for (int p = 0; p < N; ++p)
-        *reinterpret_cast<u32x4 *>(value_ws + (unit + lower_block(w, ks) * N + p) * kUnit + lane * 16) = f[p];
-    }
-  };
-  rows_out(std::integral_constant<int, 2>{}, 0);
-  wave_fence();
-  // A wave's rows of T are its own from here: P takes their place.
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * j + lr] = qk[j][i];
-  wave_fence();
-  rows_out(std::integral_constant<int, OPL>{}, U::P);
 }
 
 // ---------------------------------------------------------------------------
@@ -1308,7 +1349,9 @@ static void launch_scan(unsigned grid, hipStream_t s, const PrefillArgs &a) {
 }
 template <typename A, typename Out, int KP>
 static void launch_prefill_dims(int nw, unsigned scan_grid, hipStream_t s, const PrefillArgs &a) {
-  hipLaunchKernelGGL((prepare_kernel<A, Out, KP>), dim3(unsigned(a.slots) * unsigned(a.HV)), dim3(kPrepareThreads), 0, s, a);
+  const dim3 grid(unsigned(a.slots) * unsigned(a.H));
+  if (a.ratio == 1) hipLaunchKernelGGL((prepare_kernel<A, Out, KP, 1>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((prepare_kernel<A, Out, KP, 2>), grid, dim3(512), 0, s, a);
   if (nw == 0) {
     hipLaunchKernelGGL((scan_split_kernel<A, Out, KP>), dim3(scan_grid), dim3(kSplitThreads), 0, s, a);
     return;
