@@ -105,6 +105,12 @@ __host__ __device__ __forceinline__ int slot_of(bool align, int block, int b, in
   return align ? first_token / kChunk + int(unsigned(first_token) / unsigned(block)) + 3 * b : first_token / kChunk + b;
 }
 
+// Waits for every load. Before a loop that counts its loads in flight: the
+// compiler's counts hold for the first round as well as for the others, and a
+// first round with fewer loads behind the one waited for would make every round
+// wait for the stores and loads it has more.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
 // Orders LDS across the workgroup without draining global loads in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 __device__ __forceinline__ void wave_fence() {
@@ -183,7 +189,8 @@ __device__ __forceinline__ float inverse_power(float x) {
 // Whether a column's largest value needs no other scale, and the factor that
 // brings one past F16's reach back inside.
 __device__ __forceinline__ bool column_fits(float m) {
-  return m == 0.0f || !(m < kColumnLeast || m > kColumnMost) || m > 3e38f;
+  // Bitwise: as shortcuts these would be branches of the lanes.
+  return (m == 0.0f) | ((m >= kColumnLeast) & (m <= kColumnMost)) | !(m <= 3e38f);
 }
 __device__ __forceinline__ float back_inside(float m) { return m > 32768.0f ? kColumnAim * inverse_power(m) : 1.0f; }
 
@@ -1018,6 +1025,7 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     float check_next = load_check();
     load_p();
     f32x4 mul = scalars(kScMul);
+    loads_done();
     while (true) {
       const int done_next = done + n, in_next = after(inside, n);
       const bool more = done_next < r.n;
@@ -1118,11 +1126,23 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     if constexpr (EB == 4) return __uint_as_float(bits);
     else return to_f32(__builtin_bit_cast(A, uint16_t(bits)));
   };
+  // A wave's S tiles make OWN of the KS operands of K S0^T in its own registers:
+  // it starts with those, before the others' have come round.
+  constexpr int OWN = KT / 2;
+  uint32_t k_at[KS], s_at[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    const int ks = (w * OWN + i) % KS;
+    k_at[i] = lane_at + ks * PL * kUnit;
+    s_at[i] = lane_at + ks * kUnit;
+  }
   const char *kp = key_ws + w * KS * PL * kUnit, *ktp = key_ws + (U::KT + w * KT * 2 * PL) * kUnit;
   const char *tp = value_ws + lower_block(w, 0) * 2 * kUnit;
   const auto load_k = [&]() {
 #pragma unroll
-    for (int i = 0; i < KS * PL; ++i) kf[i / PL][i % PL] = operand(kp, i);
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int p = 0; p < PL; ++p) kf[i][p] = *reinterpret_cast<const u32x4 *>(kp + k_at[i] + p * kUnit);
   };
   const auto load_t = [&]() {
 #pragma unroll
@@ -1165,17 +1185,31 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     unscale /= f;
   };
   // Planes of the wave's S tiles, in operand order: tile i is half i % 2 of
-  // columns 32 (i / 2) ...
+  // columns 32 (i / 2) .. . X starts with what is at hand.
+  f32x4 X[2];
   const auto publish_s = [&]() {
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      const int tile = w * KT + i;
+    X[0] = X[1] = f32x4{0, 0, 0, 0};
+    if constexpr (OWN == 0) {
       uint32_t lo[2], hi[2];
-      split2<2>(S[i][0], S[i][1], lo);
-      split2<2>(S[i][2], S[i][3], hi);
+      split2<2>(S[0][0], S[0][1], lo);
+      split2<2>(S[0][2], S[0][3], hi);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
-        *reinterpret_cast<u32x2 *>(&Sp[p][tile >> 1][lane_at + (tile & 1) * 8]) = u32x2{lo[p], hi[p]};
+        *reinterpret_cast<u32x2 *>(&Sp[p][w >> 1][lane_at + (w & 1) * 8]) = u32x2{lo[p], hi[p]};
+    } else {
+      u32x4 own[OWN > 0 ? OWN : 1][2];
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        split8<2>(S[2 * i], S[2 * i + 1], own[i]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4 *>(&Sp[p][0][0] + s_at[i]) = own[i][p];
+      }
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        X[0] = mfma(kf[i][0], own[i][0], X[0]);
+        X[1] = mfma(kf[i][0], own[i][1], X[1]);
+        if constexpr (PL == 2) X[1] = mfma(kf[i][1], own[i][0], X[1]);
+      }
     }
   };
   const uint32_t row_at = (w >> 1) * kUnit + lane_at + (w & 1) * 8;
@@ -1201,12 +1235,7 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     publish_top(largest(0.0f, f32x4{16.0f * ms, 64.0f * sigma * mv, 0.0f, 0.0f}), top_s);
   };
 
-  load_k();
-  f32x4 in_scale = scalars(kScIn);
   load_v(n, vv);
-  // The next two chunks' tokens: their lengths are needed as their loads start.
-  int in_1 = after(inside, n), n_1 = n < r.n ? length(n, in_1) : 0;
-  load_v(n_1, v_next);
 #pragma unroll
   for (int i = 0; i < KT; ++i) {
     S[i] = f32x4{0, 0, 0, 0};
@@ -1214,10 +1243,16 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
   }
+  // In the order of the loop: a wait counts the loads behind the one it is for.
+  f32x2 end_check = load_end();
+  load_k();
+  f32x4 in_scale = scalars(kScIn);
+  // The next two chunks' tokens: their lengths are needed as their loads start.
+  int in_1 = after(inside, n), n_1 = n < r.n ? length(n, in_1) : 0;
+  load_v(n_1, v_next);
   load_t();
   f32x4 out_decay = scalars(kScOut);
-  load_kt();
-  f32x2 end_check = load_end();
+  loads_done();
   top_state(vv);
   publish_s();
 
@@ -1226,27 +1261,29 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     const bool more = done_next < r.n;
     const int in_2 = after(in_1, n_1), n_2 = done_2 < r.n ? length(done_2, in_2) : 0;
     const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
-    kp += kstep;
-    ktp += kstep;
-    tp += vstep;
-    sc += vstep;
     const float end = end_check[0];
     const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(end_check[1])) != 0;
-    // First of the next chunk's loads, because it is the first to be waited for.
-    end_check = load_end();
     lds_barrier();
     // Planes are read before the columns' sizes are looked at, and again where
-    // those call for it.
+    // those call for it. Loads from memory go out while LDS answers: a wave that
+    // waits for their path to take them would otherwise hold the chain up.
     u32x4 sp[KS][2];
     const auto read_s = [&]() {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int i = OWN; i < KS; ++i)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) sp[ks][p] = shared(Sp[p][ks]);
+        for (int p = 0; p < 2; ++p) sp[i][p] = *reinterpret_cast<const u32x4 *>(&Sp[p][0][0] + s_at[i]);
     };
+    const float m = top(top_s);
+    read_s();
+    asm volatile("" ::: "memory");  // reads stay above the branch
+    load_kt();
+    ktp += kstep;
+    kp += kstep;
+    tp += vstep;
+    sc += vstep;
+    end_check = load_end();
     {
-      const float m = top(top_s);
-      read_s();
       const bool fits = column_fits(m);
       if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
         rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
@@ -1256,24 +1293,18 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
       }
     }
     // X = K S0^T.
-    f32x4 X[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      X[0] = mfma(kf[ks][0], sp[ks][0], X[0]);
-      X[1] = mfma(kf[ks][0], sp[ks][1], X[1]);
-      if constexpr (PL == 2) X[1] = mfma(kf[ks][1], sp[ks][0], X[1]);
+    for (int i = OWN; i < KS; ++i) {
+      X[0] = mfma(kf[i][0], sp[i][0], X[0]);
+      X[1] = mfma(kf[i][0], sp[i][1], X[1]);
+      if constexpr (PL == 2) X[1] = mfma(kf[i][1], sp[i][0], X[1]);
     }
-    load_k();
     // R = v - diag(e^G) X.
     f32x4 R;
 #pragma unroll
     for (int i = 0; i < 4; ++i) R[i] = fmaf(-in_scale[i], X[0][i] + X[1][i], sigma * value(vv[i]));
     publish_rows(R, two, &Rp[0][0][0]);
     if (check) publish_top(largest(0.0f, R), top_r);
-    in_scale = scalars(kScIn);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vv[i] = v_next[i];
-    load_v(n_2, v_next);
     lds_barrier();
     if (check) {
       const float f = back_inside(top(top_r));
@@ -1284,25 +1315,30 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     }
     // c = T R, d = diag(e^{G_end - G}) c.
     f32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    {
-      const u32x4 hi = shared(Rp[0][0]), lo = shared(Rp[1][0]);
-      c[0] = mfma(tf[0][0], hi, c[0]);
-      c[1] = mfma(tf[0][1], hi, c[1]);
-      c[1] = mfma(tf[0][0], lo, c[1]);
-    }
+    u32x4 rp[2][2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) rp[0][p] = shared(Rp[p][0]);
+    if (low)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) rp[1][p] = shared(Rp[p][1]);
+    load_k();
+    in_scale = scalars(kScIn);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vv[i] = v_next[i];
+    load_v(n_2, v_next);
+    c[0] = mfma(tf[0][0], rp[0][0], c[0]);
+    c[1] = mfma(tf[0][1], rp[0][0], c[1]);
+    c[1] = mfma(tf[0][0], rp[0][1], c[1]);
     if (low) {
-      const u32x4 hi = shared(Rp[0][1]), lo = shared(Rp[1][1]);
-      c[0] = mfma(tf[1][0], hi, c[0]);
-      c[1] = mfma(tf[1][1], hi, c[1]);
-      c[1] = mfma(tf[1][0], lo, c[1]);
+      c[0] = mfma(tf[1][0], rp[1][0], c[0]);
+      c[1] = mfma(tf[1][1], rp[1][0], c[1]);
+      c[1] = mfma(tf[1][0], rp[1][1], c[1]);
     }
-    load_t();
     c[0] += c[1];
     f32x4 d = c[0] * out_decay;
     publish_rows(d, two, &Dp[0][0][0]);
     publish_rows(c[0], out_pl, &Cp[0][0][0]);
     if (check) publish_top(largest(largest(0.0f, c[0]), d), top_c);
-    out_decay = scalars(kScOut);
     lds_barrier();
     if (check) {
       const float f = back_inside(top(top_c));
@@ -1312,20 +1348,25 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
       lds_barrier();
     }
     // S1 = e^{G_end} S0 + K^T d.
+    u32x4 dp[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) dp[ks][p] = shared(Dp[p][ks]);
+    load_t();
+    out_decay = scalars(kScOut);
 #pragma unroll
     for (int i = 0; i < KT; ++i) S[i] *= end;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const u32x4 hi = shared(Dp[0][ks]), lo = shared(Dp[1][ks]);
 #pragma unroll
-      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], hi, S[i]);
+      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][0], S[i]);
 #pragma unroll
-      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], lo, S[i]);
+      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][1], S[i]);
       if constexpr (PL == 2)
 #pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][1], hi, S[i]);
+        for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][1], dp[ks][0], S[i]);
     }
-    load_kt();
     if (!more) break;
     publish_s();
     top_state(vv);
