@@ -1,9 +1,24 @@
 // C entry points of the chunked gated delta rule: checks, workspace, dispatch
 // (kernels in prefill_kernel.cuh, instantiated in prefill_*.hip).
-#include <cstdlib>
 #include "prefill_kernel.cuh"
 
 namespace gdn {
+
+// Waves a workgroup of the scan, 0 for the split scan, by the number of its
+// column tiles. A compute unit holds one workgroup of any form, so 256 at a time
+// run the chain of chunks: 256 tiles split, 1024 or 2048 at 4 or 8 waves, and a
+// round of the split scan takes about half the time of one at 4 waves. Whole
+// call, rows of 2048 tokens, BF16, K = 128, us split / 4 waves / 8 waves: 256
+// tiles 70 / 109 / 128, 512 128 / 129 / 146, 768 203 / 157 / 177, 1024 291 /
+// 193 / 209, 1280 379 / 298 / 234, 2304 665 / 483 / 435. Where two chunks'
+// operands do not fit LDS, waves of scan_kernel read them from memory, each for
+// itself, split / 4 waves: BF16, K = 256, 512 tiles 199 / 674, 2048 918 / 1359;
+// FP32, K = 128, 1024 tiles 465 / 573, 2048 904 / 803; FP32, K = 256, 512 tiles
+// 734 / 1245, 1024 1428 / 1351, 2048 2804 / 1678.
+static int scan_waves(bool staged, int planes, int64_t tiles) {
+  if (staged) return tiles <= 512 ? 0 : tiles <= 1024 ? 4 : 8;
+  return planes == 1 || tiles <= 1024 ? 0 : 4;
+}
 
 struct PrefillPlan {
   int kp, pl, opl, nw;
@@ -46,8 +61,7 @@ static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &
   p.key_bytes = slots * H * (12 * (p.kp / 32) * p.pl) * kUnit;
   p.bytes = p.key_bytes + slots * HV * (14 + 6 * p.opl) * kUnit;
   const int64_t tiles = rp.rows * HV * ((V + 15) / 16);
-  p.nw = tiles <= 1024 ? 0 : !scan_staged(p.pl, p.opl, p.kp) ? 4 : 8;
-  if (const char *e = getenv("PF_NW")) p.nw = atoi(e);
+  p.nw = scan_waves(scan_staged(p.pl, p.opl, p.kp), p.pl, tiles);
   const int per = 16 * (p.nw ? p.nw : 1);
   a.slices = int32_t((V + per - 1) / per);
   a.members = a.ratio * a.slices;

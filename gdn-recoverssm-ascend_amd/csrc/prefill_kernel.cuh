@@ -87,14 +87,28 @@ struct Units {
 // Block (token tile, 32 columns) of T and P.
 __host__ __device__ constexpr int lower_block(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
 // Scalars of a (slot, value head): arrays of 64 floats.
-enum { kScIn = 0, kScQ = 1, kScOut = 2, kScMul = 3, kScEnd = 4 };  // kScEnd: e^{G_end}, then whether to check
+enum { kScIn = 0, kScQ = 1, kScOut = 2, kScMul = 3, kScEnd = 4 };
+// The array kScEnd: e^{G_end}; whether the chunk has to be checked (below), 2
+// where its decays leave F16's range, so that it has to be walked; nothing; and
+// at 4 .. 7, where checked, whether a tile of token rows' T or P left it.
+constexpr float kOperandMost = 16384.0f;
+// A checked chunk without a step (beta |k|, with K's scale taken out) of this
+// size has corrections so far under v that little of them is left in F16.
+constexpr float kSmallStep = 0x1p-6f;
+// T stands 2^10 times as large in its planes: what a steep decay leaves of a
+// large state still counts in corrections of smaller values after it.
+constexpr float kTUp = 0x1p10f, kTDown = 0x1p-10f;
 // A column's largest value (see scan_kernel) that fits F16 through a chunk
 // whose rule is stable: no growing decay, 0 <= beta <= 2, |k| <= 2 and beta
 // |k|^2 <= 2. The step then does not stretch the state, |S| <= 16 max|S0| + 64
 // beta |k| max|v| in a column's 2-norm, and with both terms at most kColumnMost
 // the corrections, also times |k|, stay under 2 (kColumnMost + 2 kColumnMost) +
-// 2^8 < 2^16. Other chunks are checked value by value.
-constexpr float kColumnMost = 8192.0f, kColumnLeast = 64.0f, kColumnAim = 1024.0f;
+// 2^8 < 2^16. Other chunks are checked value by value. What F16 cannot hold at
+// all is walked token by token in FP32: chunks whose T, P or decays leave its
+// range, and columns in which four tokens' values all lie under kColumnSpan of
+// the largest (a plane's step is 2^-24), or in which a state 64 times as large
+// as any of them decays under kSteep.
+constexpr float kColumnMost = 8192.0f, kColumnLeast = 256.0f, kColumnAim = 1024.0f, kColumnSpan = 0x1p-16f, kSteep = 0x1p-6f;
 
 // Row b's chunks start at slot first / 64 + b, and where they start anywhere in
 // a block at first / 64 + first / block + 3 b. That leaves n tokens room for
@@ -191,6 +205,13 @@ __device__ __forceinline__ float inverse_power(float x) {
 __device__ __forceinline__ bool column_fits(float m) {
   // Bitwise: as shortcuts these would be branches of the lanes.
   return (m == 0.0f) | ((m >= kColumnLeast) & (m <= kColumnMost)) | !(m <= 3e38f);
+}
+// The lanes where column_fits, infinities aside; m is not negative, so its bits
+// compare as it does.
+__device__ __forceinline__ uint64_t inside_window(float m) {
+  return __builtin_amdgcn_ballot_w64(__float_as_uint(m) - __float_as_uint(kColumnLeast) <=
+                                     __float_as_uint(kColumnMost) - __float_as_uint(kColumnLeast)) |
+         __builtin_amdgcn_ballot_w64(m == 0.0f);
 }
 __device__ __forceinline__ float back_inside(float m) { return m > 32768.0f ? kColumnAim * inverse_power(m) : 1.0f; }
 
@@ -311,7 +332,8 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
       sq = sum_quarters(sq);
     }
     if (lq == 0) {
-      const float mul = a.l2norm ? 1.0f / sqrtf(sq + 1e-6f * div * div) : 1.0f / div;
+      // A row of zeros counts for nothing, and times 0 it stays in range.
+      const float mul = top == 0.0f ? 0.0f : a.l2norm ? 1.0f / sqrtf(sq + 1e-6f * div * div) : 1.0f / div;
       (is_q ? qmul : kmul)[row] = mul;
       if (!is_q) knorm[row] = sq * mul * mul;
     }
@@ -383,20 +405,25 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
     const double G = wave_prefix(double(g) * 1.4426950408889634);
     const float Gh = float(G), Gl = float(G - double(Gh));
     const float qscale = qmul[lane] * a.scale, qdown = inverse_power(qscale);
-    const float bk = beta * kmul[lane], qn = qscale * qdown, km = kmul[lane];
+    const float km = kmul[lane], bk = beta * km, qn = qscale * qdown;
+    const float k2 = knorm[lane];
+    const bool unstable = __builtin_amdgcn_ballot_w64(!(g <= 0.0f && beta >= 0.0f && beta <= 2.0f && k2 <= 4.0f &&
+                                                        beta * k2 <= 2.0f)) != 0;
     if (w == 0 && works) {
       const double end = __shfl(G, 63);
       float *sc = reinterpret_cast<float *>(value_ws + U::SC * kUnit);
-      const float e = __builtin_amdgcn_exp2f(Gh + Gl);
+      const float e = __builtin_amdgcn_exp2f(Gh + Gl), down = __builtin_amdgcn_exp2f(float(end - G));
       sc[kScIn * 64 + lane] = e * km;
       // The outputs' own scale: a power of two near Q's row, so that P fits F16.
       sc[kScQ * 64 + lane] = e * qn;
-      sc[kScOut * 64 + lane] = __builtin_amdgcn_exp2f(float(end - G)) * km;
+      sc[kScOut * 64 + lane] = down;
       sc[kScMul * 64 + lane] = 1.0f / qdown;
-      const float k2 = knorm[lane];
-      const bool stable = g <= 0.0f && beta >= 0.0f && beta <= 2.0f && k2 <= 4.0f && beta * k2 <= 2.0f;
-      const bool check = __builtin_amdgcn_ballot_w64(!stable) != 0;
-      sc[kScEnd * 64 + lane] = lane == 0 ? __builtin_amdgcn_exp2f(float(end)) : check ? 1.0f : 0.0f;
+      const bool wild = __builtin_amdgcn_ballot_w64(!(e <= kOperandMost && down <= kOperandMost)) != 0 ||
+                        __builtin_amdgcn_ballot_w64(fabsf(bk) >= kSmallStep) == 0;
+      if (lane < 2) {
+        const float check = !unstable ? 0.0f : wild ? 2.0f : 1.0f;
+        sc[kScEnd * 64 + lane] = lane == 0 ? __builtin_amdgcn_exp2f(float(end)) : check;
+      }
     }
     // L and P, token rows 16w + 4 lq + i, columns 16j + lr. Off the diagonal
     // e^{G_t - G_s} is e^{G_t - G_r} e^{G_r - G_s} with r the block's last
@@ -407,7 +434,7 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
       const int t = 16 * w + 4 * lq + i;
       Ght[i] = __shfl(Gh, t);
       Glt[i] = __shfl(Gl, t);
-      bt[i] = __shfl(bk, t);
+      bt[i] = __shfl(bk * km, t);
       qt[i] = __shfl(qn, t);
     }
     f32x4 P[4];
@@ -418,7 +445,7 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
       f32x4 L = {0, 0, 0, 0};
       if (j < w) {
         const float Ghr = __shfl(Gh, 16 * j + 15), Glr = __shfl(Gl, 16 * j + 15);
-        const float col = __builtin_amdgcn_exp2f((Ghr - __shfl(Gh, s)) + (Glr - __shfl(Gl, s))) * __shfl(km, s);
+        const float col = __builtin_amdgcn_exp2f((Ghr - __shfl(Gh, s)) + (Glr - __shfl(Gl, s)));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghr) + (Glt[i] - Glr)) * col;
@@ -426,11 +453,11 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
           P[j][i] = qt[i] * d * qk[j][i];
         }
       } else if (j == w) {
-        const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s), kms = __shfl(km, s);
+        const float Ghs = __shfl(Gh, s), Gls = __shfl(Gl, s);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = 4 * lq + i;
-          const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghs) + (Glt[i] - Gls)) * kms;
+          const float d = __builtin_amdgcn_exp2f((Ght[i] - Ghs) + (Glt[i] - Gls));
           L[i] = lr < t ? bt[i] * d * kk[j][i] : 0.0f;
           P[j][i] = lr <= t ? qt[i] * d * qk[j][i] : 0.0f;
         }
@@ -509,13 +536,18 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
       }
     }
     __syncthreads();
-    const float bs = __shfl(beta, 16 * w + lr);
+    const float bs = __shfl(bk, 16 * w + lr) * kTUp;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
       if (w + d < 4)
 #pragma unroll
         for (int i = 0; i < 4; ++i) Ls[16 * (w + d) + 4 * lq + i][16 * w + lr] = T[d][i] * bs;
     __syncthreads();
+    float top_t = 0.0f;  // of the wave's token rows
+    if (unstable)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= w) top_t = largest(top_t, *reinterpret_cast<const f32x4 *>(&Ls[16 * w + lr][16 * j + 4 * lq]));
     // Rows of T, then of P, as operands.
     const auto rows_out = [&](auto planes, int unit) {
       constexpr int N = decltype(planes)::value;
@@ -540,6 +572,16 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
       for (int i = 0; i < 4; ++i) Ls[16 * w + 4 * lq + i][16 * j + lr] = P[j][i];
     wave_fence();
     rows_out(std::integral_constant<int, OPL>{}, U::P);
+    if (unstable) {
+      float m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = largest(m, P[j]);
+      if (!works) m = 0.0f;
+      const bool out_of_range = m > kOperandMost || top_t > kOperandMost;
+      const bool any = __builtin_amdgcn_ballot_w64(out_of_range) != 0;
+      if (works && lane == 0)
+        reinterpret_cast<float *>(value_ws + U::SC * kUnit)[kScEnd * 64 + 4 + w] = any ? 1.0f : 0.0f;
+    }
     wave_fence();
   }
 }
@@ -586,6 +628,161 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_buffer(const void *p, 
                                            __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
+// One token's gates and norms for the walk of a chunk token by token.
+struct Walk {
+  GateParams gates;
+  const PrefillArgs &a;
+  int hv, h;
+  __device__ __forceinline__ Walk(const PrefillArgs &args, int hv_, int h_)
+      : gates(load_gates(args.a_log, args.dt_bias, args.gating, args.gated != 0, hv_)), a(args), hv(hv_), h(h_) {}
+  __device__ __forceinline__ float decay(int64_t tok) const {
+    return expf(log_decay(gates, load_as_f32(a.g, tok * a.g_ts + hv, a.g_dt)));
+  }
+  __device__ __forceinline__ float beta(int64_t tok) const {
+    return beta_of(gates, load_as_f32(a.beta, tok * a.beta_ts + hv, a.beta_dt));
+  }
+  __device__ __forceinline__ float norm(float sq) const { return a.l2norm ? 1.0f / sqrtf(sq + 1e-6f) : 1.0f; }
+  // Columns k0 .. k0 + 3 of a token's K or Q.
+  template <typename A>
+  __device__ __forceinline__ f32x4 row4(const void *p, int64_t ts, int64_t tok, int k0) const {
+    f32x4 x = {0, 0, 0, 0};
+    if (k0 < a.K) {
+      A raw[4];
+      __builtin_memcpy(raw, static_cast<const A *>(p) + tok * ts + int64_t(h) * a.K + k0, sizeof(raw));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = to_f32(raw[e]);
+    }
+    return x;
+  }
+};
+constexpr int kWalkSums = 5 * 16 * 4;  // floats: a sum, a column, a wave
+// What a token needs of the state as it stands: S k, S q, |k|^2, |q|^2, k.q.
+struct WalkSums {
+  float sk = 0, sq = 0, kk = 0, qq = 0, kq = 0;
+  __device__ __forceinline__ void add(const f32x4 &S, const f32x4 &k, const f32x4 &q) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sk = fmaf(S[e], k[e], sk);
+      sq = fmaf(S[e], q[e], sq);
+      kk = fmaf(k[e], k[e], kk);
+      qq = fmaf(q[e], q[e], qq);
+      kq = fmaf(k[e], q[e], kq);
+    }
+  }
+  __device__ __forceinline__ void over_quarters() {
+    sk = sum_quarters(sk), sq = sum_quarters(sq), kk = sum_quarters(kk), qq = sum_quarters(qq), kq = sum_quarters(kq);
+  }
+};
+
+// A chunk's tokens one after the other, from the inputs themselves: the state
+// (as it is, unscaled) and the outputs of this wave's 16 columns, lanes as in
+// scan_kernel. Not inlined, so that the loops around the call keep their
+// registers; the launch's arguments are read where they were passed.
+template <int N>
+struct WalkState {
+  f32x4 s[N];
+};
+__device__ __forceinline__ const PrefillArgs &launch_arguments(const void *p) {
+  return *reinterpret_cast<const PrefillArgs *>(uniform64(int64_t(reinterpret_cast<uintptr_t>(p))));
+}
+template <typename A, typename Out, int NT>
+__device__ __attribute__((noinline)) WalkState<NT> walk_chunk(WalkState<NT> state, const void *args, int first, int n,
+                                                              int hv, int h, int v0) {
+  const PrefillArgs &a = launch_arguments(args);
+  first = __builtin_amdgcn_readfirstlane(first), n = __builtin_amdgcn_readfirstlane(n);
+  hv = __builtin_amdgcn_readfirstlane(hv), h = __builtin_amdgcn_readfirstlane(h);
+  const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+  const bool column = v0 + lr < a.V;
+  const int64_t col = int64_t(hv) * a.V + v0 + lr;
+  const Walk at(a, hv, h);
+#pragma clang loop unroll(disable)
+  for (int t = 0; t < n; ++t) {
+    const int64_t tok = first + t;
+    WalkSums sums;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      sums.add(state.s[i], at.row4<A>(a.k, a.k_ts, tok, 16 * i + 4 * lq), at.row4<A>(a.q, a.q_ts, tok, 16 * i + 4 * lq));
+    sums.over_quarters();
+    const float d = at.decay(tok), rk = at.norm(sums.kk);
+    const float x = column ? to_f32(static_cast<const A *>(a.v)[tok * a.v_ts + col]) : 0.0f;
+    const float c = at.beta(tok) * (x - d * rk * sums.sk);
+    if (column && lq == 0)
+      static_cast<Out *>(a.out)[tok * a.out_ts + col] =
+          from_f32<Out>(a.scale * at.norm(sums.qq) * fmaf(d, sums.sq, c * rk * sums.kq));
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      state.s[i] = state.s[i] * d + at.row4<A>(a.k, a.k_ts, tok, 16 * i + 4 * lq) * (c * rk);
+  }
+  return state;
+}
+// The same where the four waves of a chain hold a quarter of the columns of K
+// each; every wave of the workgroup passes a barrier a token.
+template <typename A, typename Out, int KT>
+__device__ __attribute__((noinline)) WalkState<KT> walk_chunk_split(WalkState<KT> state, const void *args,
+                                                                    float *sums_of, int first, int n, int hv, int h,
+                                                                    int v0) {
+  const PrefillArgs &a = launch_arguments(args);
+  first = __builtin_amdgcn_readfirstlane(first), n = __builtin_amdgcn_readfirstlane(n);
+  hv = __builtin_amdgcn_readfirstlane(hv), h = __builtin_amdgcn_readfirstlane(h);
+  const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool column = v0 + lr < a.V;
+  const int64_t col = int64_t(hv) * a.V + v0 + lr;
+  const Walk at(a, hv, h);
+#pragma clang loop unroll(disable)
+  for (int t = 0; t < n; ++t) {
+    const int64_t tok = first + t;
+    f32x4 k[KT];
+    WalkSums own;
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      const int k0 = 16 * (w * KT + i) + 4 * lq;
+      k[i] = at.row4<A>(a.k, a.k_ts, tok, k0);
+      own.add(state.s[i], k[i], at.row4<A>(a.q, a.q_ts, tok, k0));
+    }
+    own.over_quarters();
+    // Two sets: a wave is at most one token ahead of the slowest.
+    float *const sums = sums_of + (t & 1) * kWalkSums + lr * 4;
+    if (lq == 0) {
+      sums[w] = own.sk, sums[64 + w] = own.sq;
+      sums[128 + w] = own.kk, sums[192 + w] = own.qq, sums[256 + w] = own.kq;
+    }
+    lds_barrier();
+    const auto total = [&](int i) {
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(sums + 64 * i);
+      return (x[0] + x[1]) + (x[2] + x[3]);
+    };
+    const float d = at.decay(tok), rk = at.norm(total(2));
+    const float x = column ? to_f32(static_cast<const A *>(a.v)[tok * a.v_ts + col]) : 0.0f;
+    const float c = at.beta(tok) * (x - d * rk * total(0));
+    if (column && lq == 0 && w == 0)
+      static_cast<Out *>(a.out)[tok * a.out_ts + col] =
+          from_f32<Out>(a.scale * at.norm(total(3)) * fmaf(d, total(1), c * rk * total(4)));
+#pragma unroll
+    for (int i = 0; i < KT; ++i) state.s[i] = state.s[i] * d + k[i] * (c * rk);
+  }
+  return state;
+}
+// The smaller of m and the largest of four values, if that is not zero.
+__device__ __forceinline__ float least_top(float m, float top) { return fminf(m, top == 0.0f ? INFINITY : top); }
+__device__ __forceinline__ float min_quarters(float x) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fminf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fminf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+// The largest 16 |S| of a column up to which its chunk need not be walked, by
+// its V: 64 max|v|, and the smallest of its fours' 64 max|v|.
+__device__ __forceinline__ float state_limit(float value, float least, bool steep) {
+  const float span = least < kColumnSpan * value ? -1.0f : least * (1.0f / kColumnSpan);
+  return (steep & (value != 0.0f)) ? fminf(span, 16.0f * value) : span;
+}
+// Whether the chunk at these scalars has to be walked; `check` as prepare left it.
+__device__ __forceinline__ bool walked(float check, const f32x4 &tiles) {
+  // Tiles count where the chunk is checked at all.
+  return (check == 2.0f) | ((check == 1.0f) & (largest(0.0f, tiles) != 0.0f));
+}
+
 // Whether two chunks' operands fit LDS; else waves read them from memory.
 constexpr bool scan_staged(int pl, int opl, int kp) { return 2 * (12 * (kp / 32) * pl + 14 + 6 * opl) <= 160; }
 
@@ -599,7 +796,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   constexpr bool STAGED = scan_staged(PL, OPL, KP);
   constexpr int KS = KP / 32, NT = KP / 16, EB = int(sizeof(A)), UNITS = U::KEY + U::VALUE;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // STAGED: two chunks' operands
-  const int lane = threadIdx.x & 63, wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lq = lane >> 4;
   // Workgroups of one key head's group (they read the same K and Q) sit on one
   // XCD: consecutive workgroups go to the eight XCDs in turn.
@@ -623,8 +820,6 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   const char *key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit);
   const char *value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit);
   const int64_t key_step = int64_t(a.H) * (U::KEY * kUnit), value_step = int64_t(a.HV) * (U::VALUE * kUnit);
-  const uint32_t lane_at = lane * 16;
-
   // Chunk lengths from position to position.
   int done = 0, inside = a.align ? int(r.C % a.block) : 0;
   const auto length = [&](int at, int in) {
@@ -634,293 +829,340 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   };
   int n = length(0, inside);
 
-  // Operands of the current chunk, by unit.
   int buffer = 0;
-  const auto operand = [&](int u) -> u32x4 {
-    if constexpr (STAGED) return *reinterpret_cast<const u32x4 *>(lds + buffer + u * kUnit + lane_at);
-    else return *reinterpret_cast<const u32x4 *>((u < U::KEY ? key_ws + u * kUnit : value_ws + (u - U::KEY) * kUnit) + lane_at);
-  };
-  const auto scalars = [&](int array, int tile) -> f32x4 {
-    const int at = array * 256 + (tile < 0 ? 0 : (16 * tile + 4 * lq) * 4);  // tile < 0: the array's first four
-    if constexpr (STAGED) return *reinterpret_cast<const f32x4 *>(lds + buffer + (U::KEY + U::SC) * kUnit + at);
-    else return *reinterpret_cast<const f32x4 *>(value_ws + U::SC * kUnit + at);
-  };
-  // The wave's jobs of four units each, of the chunk at (key, value).
-  constexpr int KEY_GROUPS = U::KEY / 4, GROUPS = KEY_GROUPS + (U::VALUE + 3) / 4, JOBS = (GROUPS + NW - 1) / NW;
-  const uint32_t lds_base = uint32_t(uintptr_t((__attribute__((address_space(3))) char *)lds));
-  const auto stage = [&](int from, int till, const char *key, const char *value, int to) {
-    if constexpr (STAGED) {
-#pragma unroll
-      for (int j = 0; j < JOBS; ++j) {
-        if (j < from || j >= till) continue;
-        const int g = j * NW + wave;
-        const char *src = g < KEY_GROUPS ? key + g * 4 * kUnit : value + (g - KEY_GROUPS) * 4 * kUnit;
-        const uint32_t dst = lds_base + uint32_t(to + g * 4 * kUnit);
-        if (g < GROUPS - (U::VALUE % 4 == 2)) copy_units4(src, lane_at, dst);
-        else if (U::VALUE % 4 == 2 && g == GROUPS - 1) copy_units2(src, lane_at, dst);
-      }
-    }
-  };
-  stage(0, JOBS, key_ws, value_ws, 0);
-
-  // V of the chunk: rows past its n tokens lie behind the resource's end.
-  const int v_bytes = int(a.v_ts) * EB, out_bytes = int(a.out_ts) * ob;
-  const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + r.bos * a.v_ts + int64_t(hv) * a.V);
-  char *op = static_cast<char *>(a.out) + (r.bos * a.out_ts + int64_t(hv) * a.V) * ob;
-  const int v_col = column ? (v0 + lr) * EB + 4 * lq * v_bytes : kScanDead;
-  const int out_col = column ? (v0 + lr) * ob + 4 * lq * out_bytes : kScanDead;
-  uint32_t vv[4][4];
-  const auto load_v = [&](int tokens) {
-    const auto rs = uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int off = v_col + (16 * t + i) * v_bytes;
-        if constexpr (EB == 4) vv[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
-        else vv[t][i] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
-      }
-  };
-  const auto value = [&](int t, int i) {
-    if constexpr (EB == 4) return __uint_as_float(vv[t][i]);
-    else return to_f32(__builtin_bit_cast(A, uint16_t(vv[t][i])));
-  };
-  load_v(n);
-
-  const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
-    return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * i + 4 * lq;
-  };
   f32x4 S[NT];
-  float sigma = 1.0f, unscale = 1.0f;  // S, v, c and out of this lane's column stand here times sigma
+
+  // From here once, and again behind a chunk that has been walked: with the call
+  // outside the loop over the chunks, that loop keeps its registers.
+  for (bool begins = true;; begins = false) {
+    int own_lane = int(threadIdx.x) & 63;
+    asm volatile("" : "+v"(own_lane));  // nothing made of it is kept from one round to the next
+    const int lane = own_lane, lr = lane & 15, lq = lane >> 4;
+    const bool column = v0 + lr < a.V;
+    const uint32_t lane_at = lane * 16;
+    // Operands of the current chunk, by unit.
+    const auto operand = [&](int u) -> u32x4 {
+      if constexpr (STAGED) return *reinterpret_cast<const u32x4 *>(lds + buffer + u * kUnit + lane_at);
+      else return *reinterpret_cast<const u32x4 *>((u < U::KEY ? key_ws + u * kUnit : value_ws + (u - U::KEY) * kUnit) + lane_at);
+    };
+    const auto scalars = [&](int array, int tile) -> f32x4 {
+      const int at = array * 256 + (tile < 0 ? 16 * (-1 - tile) : (16 * tile + 4 * lq) * 4);  // tile < 0: fours from the first
+      if constexpr (STAGED) return *reinterpret_cast<const f32x4 *>(lds + buffer + (U::KEY + U::SC) * kUnit + at);
+      else return *reinterpret_cast<const f32x4 *>(value_ws + U::SC * kUnit + at);
+    };
+    // The wave's jobs of four units each, of the chunk at (key, value).
+    constexpr int KEY_GROUPS = U::KEY / 4, GROUPS = KEY_GROUPS + (U::VALUE + 3) / 4, JOBS = (GROUPS + NW - 1) / NW;
+    const uint32_t lds_base = uint32_t(uintptr_t((__attribute__((address_space(3))) char *)lds));
+    const auto stage = [&](int from, int till, const char *key, const char *value, int to) {
+      if constexpr (STAGED) {
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    S[i] = f32x4{0, 0, 0, 0};
-    if (!r.fresh && column && 16 * i + 4 * lq < a.K)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
-  }
-  const auto store_state = [&](int64_t page) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-      if (column && 16 * i + 4 * lq < a.K) {
-        const int64_t at = state_at(page, i);
-        const f32x4 x = S[i] * unscale;
-        if (a.state_dt == GDN_DT_F32) {
-          *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
-        } else if (a.state_dt == GDN_DT_BF16) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+        for (int j = 0; j < JOBS; ++j) {
+          if (j < from || j >= till) continue;
+          const int g = j * NW + wave;
+          const char *src = g < KEY_GROUPS ? key + g * 4 * kUnit : value + (g - KEY_GROUPS) * 4 * kUnit;
+          const uint32_t dst = lds_base + uint32_t(to + g * 4 * kUnit);
+          if (g < GROUPS - (U::VALUE % 4 == 2)) copy_units4(src, lane_at, dst);
+          else if (U::VALUE % 4 == 2 && g == GROUPS - 1) copy_units2(src, lane_at, dst);
         }
       }
-  };
-  const auto rescale = [&](float f) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) S[i] *= f;
-    sigma *= f;
-    unscale /= f;
-  };
+    };
+    if (begins) stage(0, JOBS, key_ws, value_ws, 0);
 
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  while (true) {
-    if constexpr (STAGED) lds_barrier();
-    // The next chunk; where there is none, its loads repeat this one's slot and
-    // take no tokens.
-    const int done_next = done + n;
-    int in_next = inside + n;
-    in_next = in_next == a.block ? 0 : in_next;
-    const bool more = done_next < r.n;
-    const int n_next = more ? length(done_next, in_next) : 0;
-    const char *key_next = key_ws + (more ? key_step : 0), *value_next = value_ws + (more ? value_step : 0);
-    const int to = UNITS * kUnit - buffer;
-    vp += int64_t(n) * v_bytes;
-
-    // Keep this column's values inside F16.
-    const f32x4 end4 = scalars(kScEnd, -1);
-    const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(end4[1])) != 0;
-    {
-      float ms = 0.0f, mv = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) ms = largest(ms, S[i]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) mv = largest(mv, f32x4{value(t, 0), value(t, 1), value(t, 2), value(t, 3)});
-      const float m = max_quarters(fmaxf(16.0f * ms, 64.0f * sigma * mv));
-      const bool fits = column_fits(m);
-      if (__builtin_amdgcn_ballot_w64(!fits) != 0) rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
-    }
-    // X = K S0^T and Q S0^T.
-    f32x4 X[4], O[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) X[t] = O[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      u32x4 sp[2], so[OPL];
-      split8<2>(S[2 * ks], S[2 * ks + 1], sp);
-#pragma unroll
-      for (int p = 0; p < OPL; ++p) so[p] = sp[p];
-      u32x4 kf[4][PL], qf[4][PL];
+    // V of the chunk: rows past its n tokens lie behind the resource's end.
+    const int v_bytes = int(a.v_ts) * EB, out_bytes = int(a.out_ts) * ob;
+    const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + (r.bos + done) * a.v_ts + int64_t(hv) * a.V);
+    char *op = static_cast<char *>(a.out) + ((r.bos + done) * a.out_ts + int64_t(hv) * a.V) * ob;
+    const int v_col = column ? (v0 + lr) * EB + 4 * lq * v_bytes : kScanDead;
+    const int out_col = column ? (v0 + lr) * ob + 4 * lq * out_bytes : kScanDead;
+    uint32_t vv[4][4];
+    const auto load_v = [&](int tokens) {
+      const auto rs = uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          kf[t][p] = operand((t * KS + ks) * PL + p);
-          qf[t][p] = operand(U::Q + (t * KS + ks) * PL + p);
+        for (int i = 0; i < 4; ++i) {
+          const int off = v_col + (16 * t + i) * v_bytes;
+          if constexpr (EB == 4) vv[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+          else vv[t][i] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
         }
-      // Token tile by token tile for each pair of planes: a product waits for
-      // the one before it on its accumulator.
+    };
+    const auto value = [&](int t, int i) {
+      if constexpr (EB == 4) return __uint_as_float(vv[t][i]);
+      else return to_f32(__builtin_bit_cast(A, uint16_t(vv[t][i])));
+    };
+    load_v(n);
+
+    const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
+      return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * i + 4 * lq;
+    };
+    float sigma = 1.0f, unscale = 1.0f;  // S, v, c and out of this lane's column stand here times sigma
+    if (begins)
 #pragma unroll
-      for (int i = 0; i < PL; ++i)
+      for (int i = 0; i < NT; ++i) {
+        S[i] = f32x4{0, 0, 0, 0};
+        if (!r.fresh && column && 16 * i + 4 * lq < a.K)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (i + j < 2)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) X[t] = mfma(kf[t][i], sp[j], X[t]);
-#pragma unroll
-      for (int i = 0; i < PL; ++i)
-#pragma unroll
-        for (int j = 0; j < OPL; ++j)
-          if (i + j < 2)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) O[t] = mfma(qf[t][i], so[j], O[t]);
-      stage(JOBS * ks / KS, JOBS * (ks + 1) / KS, key_next, value_next, to);
-    }
-    // R = v - diag(e^G) X.
-    f32x4 R[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 in = scalars(kScIn, t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) R[t][i] = fmaf(-in[i], X[t][i], sigma * value(t, i));
-    }
-    load_v(n_next);
-    if (check) {
-      float m = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) m = largest(m, R[t]);
-      const float f = back_inside(max_quarters(m));
-      rescale(f);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        R[t] *= f;
-        O[t] *= f;
+          for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
       }
-    }
-    // c = T R.
-    f32x4 c[4];
-    {
-      u32x4 rp[2][2];
+    const auto store_state = [&](int64_t page) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) split8<2>(R[2 * ks], R[2 * ks + 1], rp[ks]);
+      for (int i = 0; i < NT; ++i)
+        if (column && 16 * i + 4 * lq < a.K) {
+          const int64_t at = state_at(page, i);
+          const f32x4 x = S[i] * unscale;
+          if (a.state_dt == GDN_DT_F32) {
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
+          } else if (a.state_dt == GDN_DT_BF16) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) c[t] = f32x4{0, 0, 0, 0};
+            for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
+          } else {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        u32x4 tf[4][2];
+            for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+          }
+        }
+    };
+    const auto rescale = [&](float f) {
 #pragma unroll
-        for (int t = 2 * ks; t < 4; ++t)
+      for (int i = 0; i < NT; ++i) S[i] *= f;
+      sigma *= f;
+      unscale /= f;
+    };
+
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    while (true) {
+      if constexpr (STAGED) lds_barrier();
+      // The next chunk; where there is none, its loads repeat this one's slot and
+      // take no tokens.
+      const int done_next = done + n;
+      int in_next = inside + n;
+      in_next = in_next == a.block ? 0 : in_next;
+      const bool more = done_next < r.n;
+      const int n_next = more ? length(done_next, in_next) : 0;
+      const char *key_next = key_ws + (more ? key_step : 0), *value_next = value_ws + (more ? value_step : 0);
+      const int to = UNITS * kUnit - buffer;
+      vp += int64_t(n) * v_bytes;
+
+      // Keep this column's values inside F16.
+      const f32x4 end4 = scalars(kScEnd, -1);
+      const float flag = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(end4[1])));
+      const bool check = flag != 0.0f;
+      {
+        float ms = 0.0f, mv = 0.0f, least = INFINITY;
 #pragma unroll
-          for (int p = 0; p < 2; ++p) tf[t][p] = operand(U::KEY + lower_block(t, ks) * 2 + p);
+        for (int i = 0; i < NT; ++i) ms = largest(ms, S[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int t = 0; t < 4; ++t) {
+          const float four = largest(0.0f, f32x4{value(t, 0), value(t, 1), value(t, 2), value(t, 3)});
+          least = least_top(least, four);
+          mv = fmaxf(mv, four);
+        }
+        ms = max_quarters(16.0f * ms);
+        mv = max_quarters(64.0f * sigma * mv);
+        least = 64.0f * sigma * min_quarters(least);
+        const float m = fmaxf(ms, mv);
+        const bool fits = column_fits(m), spans = ms <= state_limit(mv, least, end4[0] < kSteep);
+        if (check | (__builtin_amdgcn_ballot_w64(!spans) != 0))
+          if (__builtin_amdgcn_ballot_w64(!spans | walked(flag, scalars(kScEnd, -2))) != 0) break;
+        if (__builtin_amdgcn_ballot_w64(!fits) != 0) rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
+      }
+      // X = K S0^T and Q S0^T.
+      f32x4 X[4], O[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) X[t] = O[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        u32x4 sp[2], so[OPL];
+        split8<2>(S[2 * ks], S[2 * ks + 1], sp);
+#pragma unroll
+        for (int p = 0; p < OPL; ++p) so[p] = sp[p];
+        u32x4 kf[4][PL], qf[4][PL];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int p = 0; p < PL; ++p) {
+            kf[t][p] = operand((t * KS + ks) * PL + p);
+            qf[t][p] = operand(U::Q + (t * KS + ks) * PL + p);
+          }
+        // Token tile by token tile for each pair of planes: a product waits for
+        // the one before it on its accumulator.
+#pragma unroll
+        for (int i = 0; i < PL; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             if (i + j < 2)
 #pragma unroll
-              for (int t = 2 * ks; t < 4; ++t) c[t] = mfma(tf[t][i], rp[ks][j], c[t]);
+              for (int t = 0; t < 4; ++t) X[t] = mfma(kf[t][i], sp[j], X[t]);
+#pragma unroll
+        for (int i = 0; i < PL; ++i)
+#pragma unroll
+          for (int j = 0; j < OPL; ++j)
+            if (i + j < 2)
+#pragma unroll
+              for (int t = 0; t < 4; ++t) O[t] = mfma(qf[t][i], so[j], O[t]);
+        stage(JOBS * ks / KS, JOBS * (ks + 1) / KS, key_next, value_next, to);
       }
-    }
-    // d = diag(e^{G_end - G}) c.
-    f32x4 d[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) d[t] = c[t] * scalars(kScOut, t);
-    if (check) {
-      float m = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) m = largest(largest(m, c[t]), d[t]);
-      const float f = back_inside(max_quarters(m));
-      rescale(f);
+      // R = v - diag(e^G) X.
+      f32x4 R[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        c[t] *= f;
-        d[t] *= f;
-        O[t] *= f;
+        const f32x4 in = scalars(kScIn, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) R[t][i] = fmaf(-in[i], X[t][i], sigma * value(t, i));
       }
-    }
-    // S1 = e^{G_end} S0 + K^T d.
-    const float end = end4[0];
+      load_v(n_next);
+      if (check) {
+        float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) S[i] *= end;
+        for (int t = 0; t < 4; ++t) m = largest(m, R[t]);
+        const float f = back_inside(max_quarters(m));
+        rescale(f);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4 dp[2];
-      split8<2>(d[2 * ks], d[2 * ks + 1], dp);
-#pragma unroll
-      for (int i0 = 0; i0 < NT; i0 += 4) {
-        u32x4 kt[4][PL];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int p = 0; p < PL; ++p) kt[i][p] = operand(U::KT + ((i0 + i) * 2 + ks) * PL + p);
-#pragma unroll
-        for (int x = 0; x < PL; ++x)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if (x + y < 2)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) S[i0 + i] = mfma(kt[i][x], dp[y], S[i0 + i]);
+        for (int t = 0; t < 4; ++t) {
+          R[t] *= f;
+          O[t] *= f;
+        }
       }
-    }
-    // out = diag(scale e^G) Q S0^T + P c.
+      // c = T R.
+      f32x4 c[4];
+      {
+        u32x4 rp[2][2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) O[t] *= scalars(kScQ, t);
+        for (int ks = 0; ks < 2; ++ks) split8<2>(R[2 * ks], R[2 * ks + 1], rp[ks]);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4 cp[OPL], pf[4][OPL];
-      split8<OPL>(c[2 * ks], c[2 * ks + 1], cp);
+        for (int t = 0; t < 4; ++t) c[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int t = 2 * ks; t < 4; ++t)
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4 tf[4][2];
 #pragma unroll
-        for (int p = 0; p < OPL; ++p) pf[t][p] = operand(U::KEY + U::P + lower_block(t, ks) * OPL + p);
+          for (int t = 2 * ks; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < OPL; ++i)
+            for (int p = 0; p < 2; ++p) tf[t][p] = operand(U::KEY + lower_block(t, ks) * 2 + p);
 #pragma unroll
-        for (int j = 0; j < OPL; ++j)
-          if (i + j < 2)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int t = 2 * ks; t < 4; ++t) O[t] = mfma(pf[t][i], cp[j], O[t]);
-    }
-    // What was loaded for the next chunk is here; this chunk's stores then have
-    // that chunk's time.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    {
-      const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
+            for (int j = 0; j < 2; ++j)
+              if (i + j < 2)
+#pragma unroll
+                for (int t = 2 * ks; t < 4; ++t) c[t] = mfma(tf[t][i], rp[ks][j], c[t]);
+        }
+      }
+      // d = diag(e^{G_end - G}) c.
+      f32x4 d[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const f32x4 x = O[t] * (scalars(kScMul, t) * unscale);
+        c[t] *= kTDown;
+        d[t] = c[t] * scalars(kScOut, t);
+      }
+      if (check) {
+        float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int off = out_col + (16 * t + i) * out_bytes;
-          if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, off, 0, 0);
-          else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, off, 0, 0);
+        for (int t = 0; t < 4; ++t) m = largest(largest(m, c[t]), d[t]);
+        const float f = back_inside(max_quarters(m));
+        rescale(f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          c[t] *= f;
+          d[t] *= f;
+          O[t] *= f;
+        }
+      }
+      // S1 = e^{G_end} S0 + K^T d.
+      const float end = end4[0];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) S[i] *= end;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 dp[2];
+        split8<2>(d[2 * ks], d[2 * ks + 1], dp);
+#pragma unroll
+        for (int i0 = 0; i0 < NT; i0 += 4) {
+          u32x4 kt[4][PL];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int p = 0; p < PL; ++p) kt[i][p] = operand(U::KT + ((i0 + i) * 2 + ks) * PL + p);
+#pragma unroll
+          for (int x = 0; x < PL; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if (x + y < 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[i0 + i] = mfma(kt[i][x], dp[y], S[i0 + i]);
+        }
+      }
+      // out = diag(scale e^G) Q S0^T + P c.
+#pragma unroll
+      for (int t = 0; t < 4; ++t) O[t] *= scalars(kScQ, t);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x4 cp[OPL], pf[4][OPL];
+        split8<OPL>(c[2 * ks], c[2 * ks + 1], cp);
+#pragma unroll
+        for (int t = 2 * ks; t < 4; ++t)
+#pragma unroll
+          for (int p = 0; p < OPL; ++p) pf[t][p] = operand(U::KEY + U::P + lower_block(t, ks) * OPL + p);
+#pragma unroll
+        for (int i = 0; i < OPL; ++i)
+#pragma unroll
+          for (int j = 0; j < OPL; ++j)
+            if (i + j < 2)
+#pragma unroll
+              for (int t = 2 * ks; t < 4; ++t) O[t] = mfma(pf[t][i], cp[j], O[t]);
+      }
+      // What was loaded for the next chunk is here; this chunk's stores then have
+      // that chunk's time.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      {
+        const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const f32x4 x = O[t] * (scalars(kScMul, t) * unscale);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int off = out_col + (16 * t + i) * out_bytes;
+            if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, off, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, off, 0, 0);
+          }
         }
       }
       op += int64_t(n) * out_bytes;
+      if (!more) {
+        store_state(r.fin);
+        return;
+      }
+      if (a.align && in_next == 0) {
+        const int64_t page = boundary_page(a.pages, r, r.C + done_next);
+        if (page != 0) store_state(page);
+      }
+      key_ws = key_next;
+      value_ws = value_next;
+      buffer = to;
+      done = done_next;
+      inside = in_next;
+      n = n_next;
     }
-    if (!more) break;
-    if (a.align && in_next == 0) {
-      const int64_t page = boundary_page(a.pages, r, r.C + done_next);
-      if (page != 0) store_state(page);
-    }
-    key_ws = key_next;
-    value_ws = value_next;
-    buffer = to;
-    done = done_next;
-    inside = in_next;
-    n = n_next;
+    // A walked chunk; the other waves of the workgroup may be in the loop, so what
+    // the loop does for them is done here: this wave's share of the next operands.
+    rescale(unscale);
+    const int left = r.n - done - n;
+    key_ws += left > 0 ? key_step : 0;
+    value_ws += left > 0 ? value_step : 0;
+    buffer = UNITS * kUnit - buffer;
+    stage(0, JOBS, key_ws, value_ws, buffer);
+    WalkState<NT> state;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) state.s[i] = S[i];
+    const void *const args = (const void *)__builtin_amdgcn_kernarg_segment_ptr();  // the launch's only one
+    state = walk_chunk<A, Out, NT>(state, args, r.bos + done, n, hv, h, v0);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) S[i] = state.s[i];
+    done += n;
+    inside = inside + n == a.block ? 0 : inside + n;
+    const int64_t page = left == 0 ? r.fin : a.align && inside == 0 ? boundary_page(a.pages, r, r.C + done) : 0;
+    if (page != 0) store_state(page);
+    if (left == 0) return;
+    n = length(done, inside);
   }
-  store_state(r.fin);
 }
 
 // ---------------------------------------------------------------------------
@@ -942,12 +1184,13 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
     const PrefillArgs a) {
   using U = Units<A, Out, KP>;
   constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, KT = KP / 64, EB = int(sizeof(A)), ob = int(sizeof(Out));
-  // Operand planes in lane order, and per column the largest value of each
-  // chain wave.
+  // Operand planes in lane order; per column the largest value of each chain
+  // wave, and the chunk's largest 64 |v| with its state_limit.
   __shared__ __attribute__((aligned(16))) char Sp[2][KS][kUnit], Rp[2][2][kUnit], Dp[2][2][kUnit], Cp[OPL][2][kUnit];
   __shared__ __attribute__((aligned(16))) float top_s[16][4], top_r[16][4], top_c[16][4];
+  __shared__ __attribute__((aligned(16))) float tops_v[16][2], sums_of[2 * kWalkSums];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-  const int lr = lane & 15, lq = lane >> 4;
+  const int lr = lane & 15;
   const int wg = int(blockIdx.x), group = (wg / 8 / a.members) * 8 + wg % 8, member = wg / 8 % a.members;
   if (group >= a.pages.rows * a.H) return;
   const int b = group / a.H, h = group % a.H;
@@ -963,30 +1206,6 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
   }
   const int64_t slot = slot_of(a.align, a.block, b, r.bos);
   const int64_t key_step = int64_t(a.H) * (U::KEY * kUnit), value_step = int64_t(a.HV) * (U::VALUE * kUnit);
-  const char *const key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit);
-  const char *const value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit);
-  const int at4 = 16 * w + 4 * lq;
-  const bool low = w >= 2;  // T and P: columns 32 .. 63 are zero for the upper token rows
-  // Operand unit i of a wave-uniform run of units: the run's address advances in
-  // scalar registers, and every fourth unit has a lane offset of its own (an
-  // instruction's ends at 4 KB).
-  const uint32_t lane_at = lane * 16;
-  uint32_t unit_at[(KS * PL > 2 * KT * PL ? KS * PL : 2 * KT * PL) / 4 + 1];
-#pragma unroll
-  for (uint32_t i = 0; i < sizeof(unit_at) / 4; ++i) {
-    unit_at[i] = lane_at + i * 4 * kUnit;
-    asm("" : "+v"(unit_at[i]));
-  }
-  const auto operand = [&](const char *run, int i) {
-    return *reinterpret_cast<const u32x4 *>(run + unit_at[i >> 2] + (i & 3) * kUnit);
-  };
-  const char *sc = value_ws + U::SC * kUnit;
-  const uint32_t sc_at = at4 * 4;
-  const auto scalars = [&](int array) { return *reinterpret_cast<const f32x4 *>(sc + sc_at + array * 256); };
-  const auto shared = [&](const char *p) { return *reinterpret_cast<const u32x4 *>(p + lane_at); };
-  // The largest over the chain's waves of this lane's column.
-  const auto top = [&](const float (&t)[16][4]) { return largest(0.0f, *reinterpret_cast<const f32x4 *>(t[lr])); };
-
   // Chunk lengths from position to position.
   const auto length = [&](int at, int in) {
     int n = kChunk - (in & (kChunk - 1));
@@ -996,46 +1215,134 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
   const auto after = [&](int in, int n) { return in + n == a.block ? 0 : in + n; };
   int done = 0, inside = a.align ? int(r.C % a.block) : 0;
   int n = length(0, inside);
-  float sigma = 1.0f, unscale = 1.0f;
+  f32x4 S[KT];
 
-  if (wave >= 4) {
-    // ---- outputs ----
-    u32x4 qf[KS][PL], pf[2][OPL];
-    const int out_bytes = int(a.out_ts) * ob;
-    char *op = static_cast<char *>(a.out) + (r.bos * a.out_ts + int64_t(hv) * a.V) * ob;
-    int col[4];
+  // From here once, and again behind a chunk that has been walked: with the call
+  // outside the loop over the chunks, that loop keeps its registers.
+  for (int64_t chunk = 0;; ++chunk) {
+    int own_lane = int(threadIdx.x) & 63;
+    asm volatile("" : "+v"(own_lane));  // nothing made of it is kept from one round to the next
+    const int lane = own_lane, lr = lane & 15, lq = lane >> 4;
+    const bool column = v0 + lr < a.V;
+    const char *const key_ws = a.ws + (slot * a.H + h) * (U::KEY * kUnit) + chunk * key_step;
+    const char *const value_ws = a.ws_value + (slot * a.HV + hv) * (U::VALUE * kUnit) + chunk * value_step;
+    const int at4 = 16 * w + 4 * lq;
+    const bool low = w >= 2;  // T and P: columns 32 .. 63 are zero for the upper token rows
+    // Operand unit i of a wave-uniform run of units: the run's address advances in
+    // scalar registers, and every fourth unit has a lane offset of its own (an
+    // instruction's ends at 4 KB).
+    const uint32_t lane_at = lane * 16;
+    uint32_t unit_at[(KS * PL > 2 * KT * PL ? KS * PL : 2 * KT * PL) / 4 + 1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * out_bytes + (v0 + lr) * ob : kScanDead;
-    const char *qp = key_ws + (U::Q + w * KS * PL) * kUnit;
-    const char *pp = value_ws + (U::P + lower_block(w, 0) * OPL) * kUnit;
-    const auto load_q = [&]() {
-#pragma unroll
-      for (int i = 0; i < KS * PL; ++i) qf[i / PL][i % PL] = operand(qp, i);
+    for (uint32_t i = 0; i < sizeof(unit_at) / 4; ++i) {
+      unit_at[i] = lane_at + i * 4 * kUnit;
+      asm("" : "+v"(unit_at[i]));
+    }
+    const auto operand = [&](const char *run, int i) {
+      return *reinterpret_cast<const u32x4 *>(run + unit_at[i >> 2] + (i & 3) * kUnit);
     };
-    const auto load_p = [&]() {
-#pragma unroll
-      for (int p = 0; p < OPL; ++p) pf[0][p] = operand(pp, p);
-      if (low)
-#pragma unroll
-        for (int p = 0; p < OPL; ++p) pf[1][p] = operand(pp, OPL + p);
+    const char *sc = value_ws + U::SC * kUnit;
+    const uint32_t sc_at = at4 * 4;
+    const auto scalars = [&](int array) { return *reinterpret_cast<const f32x4 *>(sc + sc_at + array * 256); };
+    const auto shared = [&](const char *p) { return *reinterpret_cast<const u32x4 *>(p + lane_at); };
+    // The largest over the chain's waves of this lane's column.
+    const auto top = [&](const float (&t)[16][4]) { return largest(0.0f, *reinterpret_cast<const f32x4 *>(t[lr])); };
+
+    float sigma = 1.0f, unscale = 1.0f;  // S, v, c and out of a column stand here times sigma
+    const int v_bytes = int(a.v_ts) * EB;
+    const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + (r.bos + done) * a.v_ts + int64_t(hv) * a.V);
+    const auto value = [&](uint32_t bits) {
+      if constexpr (EB == 4) return __uint_as_float(bits);
+      else return to_f32(__builtin_bit_cast(A, uint16_t(bits)));
     };
-    const auto load_check = [&]() { return *reinterpret_cast<const float *>(sc + kScEnd * 256 + 4); };
-    load_q();
-    f32x4 scale = scalars(kScQ);
-    float check_next = load_check();
-    load_p();
-    f32x4 mul = scalars(kScMul);
-    loads_done();
-    while (true) {
-      const int done_next = done + n, in_next = after(inside, n);
-      const bool more = done_next < r.n;
-      const int n_next = more ? length(done_next, in_next) : 0;
-      const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
-      qp += kstep;
-      pp += vstep;
-      sc += vstep;
-      const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(check_next)) != 0;
-      lds_barrier();  // S0
+    // Column lr of V at four tokens `col` of a chunk of `tokens`, from vp.
+    const auto load_v4 = [&](__amdgpu_buffer_rsrc_t rs, const int (&col)[4], int tile, uint32_t *to) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int off = col[i] + 16 * tile * v_bytes;
+        if constexpr (EB == 4) to[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+        else to[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
+      }
+    };
+    const auto v_buffer = [&](int tokens) {
+      return uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
+    };
+
+
+    if (wave >= 4) {
+      // ---- outputs ----
+      u32x4 qf[KS][PL], pf[2][OPL];
+      const int out_bytes = int(a.out_ts) * ob;
+      char *op = static_cast<char *>(a.out) + ((r.bos + done) * a.out_ts + int64_t(hv) * a.V) * ob;
+      int col[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * out_bytes + (v0 + lr) * ob : kScanDead;
+      const char *qp = key_ws + (U::Q + w * KS * PL) * kUnit;
+      const char *pp = value_ws + (U::P + lower_block(w, 0) * OPL) * kUnit;
+      const auto load_q = [&]() {
+#pragma unroll
+        for (int i = 0; i < KS * PL; ++i) qf[i / PL][i % PL] = operand(qp, i);
+      };
+      const auto load_p = [&]() {
+#pragma unroll
+        for (int p = 0; p < OPL; ++p) pf[0][p] = operand(pp, p);
+        if (low)
+#pragma unroll
+          for (int p = 0; p < OPL; ++p) pf[1][p] = operand(pp, OPL + p);
+      };
+      const auto rescale = [&](float f) {
+        sigma *= f;
+        unscale /= f;
+      };
+      const auto load_check = [&]() { return *reinterpret_cast<const f32x2 *>(sc + kScEnd * 256); };
+      // The first wave, whose outputs take less than others', also looks through
+      // the V of the chunk to come.
+      uint32_t vv[4][4];
+      int v_col[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v_col[i] = column ? (4 * lq + i) * v_bytes + (v0 + lr) * EB : kScanDead;
+      const auto load_v = [&](int tokens) {
+        if (w == 0) {
+          const auto rs = v_buffer(tokens);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) load_v4(rs, v_col, j, vv[j]);
+          vp += tokens * v_bytes;
+        }
+      };
+      f32x4 tiles;
+      const auto load_tiles = [&]() {
+        if (w == 0) tiles = *reinterpret_cast<const f32x4 *>(sc + kScEnd * 256 + 16);
+      };
+      // As they are: sigma is the reader's. A limit below all where the chunk has to
+      // be walked for what prepare found.
+      const auto publish_v = [&](const f32x2 &end_check) {
+        if (w == 0) {
+          float most = 0.0f, least = INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float four = largest(0.0f, f32x4{value(vv[j][0]), value(vv[j][1]), value(vv[j][2]), value(vv[j][3])});
+            most = fmaxf(most, four);
+            least = least_top(least, four);
+          }
+          most = 64.0f * max_quarters(most);
+          least = 64.0f * min_quarters(least);
+          const float limit = walked(end_check[1], tiles) ? -1.0f : state_limit(most, least, end_check[0] < kSteep);
+          if (lq == 0) *reinterpret_cast<f32x2 *>(tops_v[lr]) = f32x2{most, limit};
+        }
+      };
+      load_v(n);
+      load_tiles();
+      publish_v(load_check());
+      int in_1 = after(inside, n), n_1 = done + n < r.n ? length(done + n, in_1) : 0;
+      load_v(n_1);
+      load_q();
+      f32x4 scale = scalars(kScQ);
+      f32x2 check_next = load_check();
+      load_p();
+      f32x4 mul = scalars(kScMul);
+      loads_done();
+      bool more, check;
+      int done_next, in_2, n_2;
       u32x4 sp[KS][OPL];
       const auto read_s = [&]() {
 #pragma unroll
@@ -1043,343 +1350,400 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
 #pragma unroll
           for (int p = 0; p < OPL; ++p) sp[ks][p] = shared(Sp[p][ks]);
       };
-      {
-        const float m = top(top_s);
+      // A chunk's start: S0 and its size. False where the chunk is walked.
+      const auto enter = [&]() -> bool {
+        done_next = done + n;
+        more = done_next < r.n;
+        in_2 = after(in_1, n_1), n_2 = done_next + n_1 < r.n ? length(done_next + n_1, in_2) : 0;
+        check = __builtin_amdgcn_readfirstlane(__float_as_int(check_next[1])) != 0;
+        qp += more ? key_step : 0;
+        pp += more ? value_step : 0;
+        sc += more ? value_step : 0;
+        check_next = load_check();
+        load_tiles();
+        lds_barrier();
+        const f32x4 tops = *reinterpret_cast<const f32x4 *>(top_s[lr]);
+        const f32x2 v_tops = *reinterpret_cast<const f32x2 *>(tops_v[lr]);
         read_s();
-        const bool fits = column_fits(m);
-        if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
-          unscale /= fits ? 1.0f : kColumnAim * inverse_power(m);
+        asm volatile("" ::: "memory");
+        const float state = largest(0.0f, tops), m = fmaxf(state, sigma * v_tops[0]);
+        const uint64_t spans = __builtin_amdgcn_ballot_w64(state <= sigma * v_tops[1]);
+        if (inside_window(m) != ~0ull) {
+          rescale(column_fits(m) ? 1.0f : kColumnAim * inverse_power(m));
           lds_barrier();
           read_s();
         }
-      }
-      f32x4 out = {0, 0, 0, 0};
+        return spans == ~0ull;
+      };
+      bool go = enter();
+      while (go) {
+        f32x4 out = {0, 0, 0, 0};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) out = mfma_planes<PL, OPL>(qf[ks], sp[ks], out);
-      load_q();
-      out *= scale;
-      scale = scalars(kScQ);
-      check_next = load_check();
-      lds_barrier();  // R
-      if (check) {
-        const float f = back_inside(top(top_r));
-        out *= f;
-        unscale /= f;
-        lds_barrier();
-      }
-      lds_barrier();  // c
-      if (check) {
-        const float f = back_inside(top(top_c));
-        out *= f;
-        unscale /= f;
-        lds_barrier();
-      }
-      {
-        u32x4 cf[OPL];
+        for (int ks = 0; ks < KS; ++ks) out = mfma_planes<PL, OPL>(qf[ks], sp[ks], out);
+        load_q();
+        out *= scale;
+        scale = scalars(kScQ);
+        lds_barrier();  // R
+        publish_v(check_next);  // of the next chunk, while there is nothing else to do
+        load_v(n_2);
+        if (check) {
+          const float f = back_inside(top(top_r));
+          out *= f;
+          rescale(f);
+          lds_barrier();
+        }
+        lds_barrier();  // c
+        if (check) {
+          const float f = back_inside(top(top_c));
+          out *= f;
+          rescale(f);
+          lds_barrier();
+        }
+        {
+          u32x4 cf[OPL];
 #pragma unroll
-        for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][0]);
-        out = mfma_planes<OPL, OPL>(pf[0], cf, out);
-      }
-      if (low) {
-        u32x4 cf[OPL];
+          for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][0]);
+          out = mfma_planes<OPL, OPL>(pf[0], cf, out);
+        }
+        if (low) {
+          u32x4 cf[OPL];
 #pragma unroll
-        for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][1]);
-        out = mfma_planes<OPL, OPL>(pf[1], cf, out);
-      }
-      load_p();
-      const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
-      const f32x4 x = out * (mul * unscale);
+          for (int p = 0; p < OPL; ++p) cf[p] = shared(Cp[p][1]);
+          out = mfma_planes<OPL, OPL>(pf[1], cf, out);
+        }
+        load_p();
+        const auto rs = uniform_buffer(op, (n - 1) * out_bytes + a.V * ob);
+        const f32x4 x = out * (mul * unscale);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, col[i], 0, 0);
-        else
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, col[i], 0, 0);
-      }
-      mul = scalars(kScMul);
-      if (!more) return;
-      op += n * out_bytes;
-      done = done_next;
-      inside = in_next;
-      n = n_next;
-    }
-  }
-
-  // ---- the chain ----
-  __builtin_amdgcn_s_setprio(2);
-  u32x4 kf[KS][PL], tf[2][2], kt[2][KT][PL];
-  uint32_t vv[4], v_next[4];  // of this chunk and the next
-  const int v_bytes = int(a.v_ts) * EB;
-  const char *vp = reinterpret_cast<const char *>(static_cast<const A *>(a.v) + r.bos * a.v_ts + int64_t(hv) * a.V);
-  int col[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * v_bytes + (v0 + lr) * EB : kScanDead;
-  const auto load_v = [&](int tokens, uint32_t (&to)[4]) {
-    const auto rs = uniform_buffer(vp, tokens > 0 ? (tokens - 1) * v_bytes + a.V * EB : 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (EB == 4) to[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, col[i], 0, 0);
-      else to[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, col[i], 0, 0);
-    }
-    vp += tokens * v_bytes;
-  };
-  const auto value = [&](uint32_t bits) {
-    if constexpr (EB == 4) return __uint_as_float(bits);
-    else return to_f32(__builtin_bit_cast(A, uint16_t(bits)));
-  };
-  // A wave's S tiles make OWN of the KS operands of K S0^T in its own registers:
-  // it starts with those, before the others' have come round.
-  constexpr int OWN = KT / 2;
-  uint32_t k_at[KS], s_at[KS];
-#pragma unroll
-  for (int i = 0; i < KS; ++i) {
-    const int ks = (w * OWN + i) % KS;
-    k_at[i] = lane_at + ks * PL * kUnit;
-    s_at[i] = lane_at + ks * kUnit;
-  }
-  const char *kp = key_ws + w * KS * PL * kUnit, *ktp = key_ws + (U::KT + w * KT * 2 * PL) * kUnit;
-  const char *tp = value_ws + lower_block(w, 0) * 2 * kUnit;
-  const auto load_k = [&]() {
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int p = 0; p < PL; ++p) kf[i][p] = *reinterpret_cast<const u32x4 *>(kp + k_at[i] + p * kUnit);
-  };
-  const auto load_t = [&]() {
-#pragma unroll
-    for (int p = 0; p < 2; ++p) tf[0][p] = operand(tp, p);
-    if (low)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) tf[1][p] = operand(tp, 2 + p);
-  };
-  const auto load_kt = [&]() {
-#pragma unroll
-    for (int i = 0; i < KT * 2 * PL; ++i) kt[i / PL % 2][i / (2 * PL)][i % PL] = operand(ktp, i);
-  };
-  const auto load_end = [&]() { return *reinterpret_cast<const f32x2 *>(sc + kScEnd * 256); };
-
-  const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
-    return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * (w * KT + i) + 4 * lq;
-  };
-  f32x4 S[KT];
-  const auto store_state = [&](int64_t page) {
-#pragma unroll
-    for (int i = 0; i < KT; ++i)
-      if (column && 16 * (w * KT + i) + 4 * lq < a.K) {
-        const int64_t at = state_at(page, i);
-        const f32x4 x = S[i] * unscale;
-        if (a.state_dt == GDN_DT_F32) {
-          *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
-        } else if (a.state_dt == GDN_DT_BF16) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (ob == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[i]), rs, col[i], 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, from_f32<Out>(x[i])), rs, col[i], 0, 0);
+        }
+        mul = scalars(kScMul);
+        go = false;
+        if (more) {
+          op += n * out_bytes;
+          done = done_next;
+          inside = in_1;
+          n = n_1;
+          in_1 = in_2;
+          n_1 = n_2;
+          ++chunk;
+          go = enter();
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+          done = r.n;
         }
       }
-  };
-  const auto rescale = [&](float f) {
-#pragma unroll
-    for (int i = 0; i < KT; ++i) S[i] *= f;
-    sigma *= f;
-    unscale /= f;
-  };
-  // Planes of the wave's S tiles, in operand order: tile i is half i % 2 of
-  // columns 32 (i / 2) .. . X starts with what is at hand.
-  f32x4 X[2];
-  const auto publish_s = [&]() {
-    X[0] = X[1] = f32x4{0, 0, 0, 0};
-    if constexpr (OWN == 0) {
-      uint32_t lo[2], hi[2];
-      split2<2>(S[0][0], S[0][1], lo);
-      split2<2>(S[0][2], S[0][3], hi);
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        *reinterpret_cast<u32x2 *>(&Sp[p][w >> 1][lane_at + (w & 1) * 8]) = u32x2{lo[p], hi[p]};
+      if (done == r.n) return;
+      for (int t = 0; t < n; ++t) lds_barrier();  // the chain makes this chunk's outputs
     } else {
-      u32x4 own[OWN > 0 ? OWN : 1][2];
+      // ---- the chain ----
+      __builtin_amdgcn_s_setprio(2);
+      u32x4 kf[KS][PL], tf[2][2], kt[2][KT][PL];
+      uint32_t vv[4], v_next[4];  // of this chunk and the next
+      int col[4];
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        split8<2>(S[2 * i], S[2 * i + 1], own[i]);
+      for (int i = 0; i < 4; ++i) col[i] = column ? (at4 + i) * v_bytes + (v0 + lr) * EB : kScanDead;
+      const auto load_v = [&](int tokens, uint32_t (&to)[4]) {
+        load_v4(v_buffer(tokens), col, 0, to);
+        vp += tokens * v_bytes;
+      };
+      // A wave's S tiles make OWN of the KS operands of K S0^T in its own registers:
+      // it starts with those, before the others' have come round.
+      constexpr int OWN = KT / 2;
+      uint32_t k_at[KS], s_at[KS];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4 *>(&Sp[p][0][0] + s_at[i]) = own[i][p];
+      for (int i = 0; i < KS; ++i) {
+        const int ks = (w * OWN + i) % KS;
+        k_at[i] = lane_at + ks * PL * kUnit;
+        s_at[i] = lane_at + ks * kUnit;
       }
+      const char *kp = key_ws + w * KS * PL * kUnit, *ktp = key_ws + (U::KT + w * KT * 2 * PL) * kUnit;
+      const char *tp = value_ws + lower_block(w, 0) * 2 * kUnit;
+      const auto load_k = [&]() {
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        X[0] = mfma(kf[i][0], own[i][0], X[0]);
-        X[1] = mfma(kf[i][0], own[i][1], X[1]);
-        if constexpr (PL == 2) X[1] = mfma(kf[i][1], own[i][0], X[1]);
-      }
-    }
-  };
-  const uint32_t row_at = (w >> 1) * kUnit + lane_at + (w & 1) * 8;
-  const auto publish_rows = [&](const f32x4 &x, auto planes, char *to) {  // to: [planes][2][kUnit]
-    constexpr int N = decltype(planes)::value;
-    uint32_t lo[N], hi[N];
-    split2<N>(x[0], x[1], lo);
-    split2<N>(x[2], x[3], hi);
+        for (int i = 0; i < KS; ++i)
 #pragma unroll
-    for (int p = 0; p < N; ++p) *reinterpret_cast<u32x2 *>(to + p * 2 * kUnit + row_at) = u32x2{lo[p], hi[p]};
-  };
-  constexpr std::integral_constant<int, 2> two{};
-  constexpr std::integral_constant<int, OPL> out_pl{};
-  const auto publish_top = [&](float m, float (&t)[16][4]) {
-    m = max_quarters(m);
-    if (lq == 0) t[lr][w] = m;
-  };
-  const auto top_state = [&](const uint32_t (&v)[4]) {
-    float ms = 0.0f;
+          for (int p = 0; p < PL; ++p) kf[i][p] = *reinterpret_cast<const u32x4 *>(kp + k_at[i] + p * kUnit);
+      };
+      const auto load_t = [&]() {
 #pragma unroll
-    for (int i = 0; i < KT; ++i) ms = largest(ms, S[i]);
-    const float mv = largest(0.0f, f32x4{value(v[0]), value(v[1]), value(v[2]), value(v[3])});
-    publish_top(largest(0.0f, f32x4{16.0f * ms, 64.0f * sigma * mv, 0.0f, 0.0f}), top_s);
-  };
+        for (int p = 0; p < 2; ++p) tf[0][p] = operand(tp, p);
+        if (low)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) tf[1][p] = operand(tp, 2 + p);
+      };
+      const auto load_kt = [&]() {
+#pragma unroll
+        for (int i = 0; i < KT * 2 * PL; ++i) kt[i / PL % 2][i / (2 * PL)][i % PL] = operand(ktp, i);
+      };
+      const auto load_end = [&]() { return *reinterpret_cast<const f32x2 *>(sc + kScEnd * 256); };
 
-  load_v(n, vv);
+      const auto state_at = [&](int64_t page, int i) {  // element offset of the lane's four k
+        return page * a.state_bs + hv * a.state_hs + int64_t(v0 + lr) * a.state_vs + 16 * (w * KT + i) + 4 * lq;
+      };
+      const auto store_state = [&](int64_t page) {
 #pragma unroll
-  for (int i = 0; i < KT; ++i) {
-    S[i] = f32x4{0, 0, 0, 0};
-    if (!r.fresh && column && 16 * (w * KT + i) + 4 * lq < a.K)
+        for (int i = 0; i < KT; ++i)
+          if (column && 16 * (w * KT + i) + 4 * lq < a.K) {
+            const int64_t at = state_at(page, i);
+            const f32x4 x = S[i] * unscale;
+            if (a.state_dt == GDN_DT_F32) {
+              *reinterpret_cast<f32x4 *>(static_cast<float *>(a.state) + at) = x;
+            } else if (a.state_dt == GDN_DT_BF16) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
-  }
-  // In the order of the loop: a wait counts the loads behind the one it is for.
-  f32x2 end_check = load_end();
-  load_k();
-  f32x4 in_scale = scalars(kScIn);
-  // The next two chunks' tokens: their lengths are needed as their loads start.
-  int in_1 = after(inside, n), n_1 = n < r.n ? length(n, in_1) : 0;
-  load_v(n_1, v_next);
-  load_t();
-  f32x4 out_decay = scalars(kScOut);
-  loads_done();
-  top_state(vv);
-  publish_s();
+              for (int e = 0; e < 4; ++e) static_cast<bf16 *>(a.state)[at + e] = from_f32<bf16>(x[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) static_cast<f16 *>(a.state)[at + e] = from_f32<f16>(x[e]);
+            }
+          }
+      };
+      const auto rescale = [&](float f) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] *= f;
+        sigma *= f;
+        unscale /= f;
+      };
+      // Planes of the wave's S tiles, in operand order: tile i is half i % 2 of
+      // columns 32 (i / 2) .. . X starts with what is at hand.
+      f32x4 X[2];
+      const auto publish_s = [&]() {
+        X[0] = X[1] = f32x4{0, 0, 0, 0};
+        if constexpr (OWN == 0) {
+          uint32_t lo[2], hi[2];
+          split2<2>(S[0][0], S[0][1], lo);
+          split2<2>(S[0][2], S[0][3], hi);
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            *reinterpret_cast<u32x2 *>(&Sp[p][w >> 1][lane_at + (w & 1) * 8]) = u32x2{lo[p], hi[p]};
+        } else {
+          u32x4 own[OWN > 0 ? OWN : 1][2];
+#pragma unroll
+          for (int i = 0; i < OWN; ++i) {
+            split8<2>(S[2 * i], S[2 * i + 1], own[i]);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) *reinterpret_cast<u32x4 *>(&Sp[p][0][0] + s_at[i]) = own[i][p];
+          }
+#pragma unroll
+          for (int i = 0; i < OWN; ++i) {
+            X[0] = mfma(kf[i][0], own[i][0], X[0]);
+            X[1] = mfma(kf[i][0], own[i][1], X[1]);
+            if constexpr (PL == 2) X[1] = mfma(kf[i][1], own[i][0], X[1]);
+          }
+        }
+      };
+      const uint32_t row_at = (w >> 1) * kUnit + lane_at + (w & 1) * 8;
+      const auto publish_rows = [&](const f32x4 &x, auto planes, char *to) {  // to: [planes][2][kUnit]
+        constexpr int N = decltype(planes)::value;
+        uint32_t lo[N], hi[N];
+        split2<N>(x[0], x[1], lo);
+        split2<N>(x[2], x[3], hi);
+#pragma unroll
+        for (int p = 0; p < N; ++p) *reinterpret_cast<u32x2 *>(to + p * 2 * kUnit + row_at) = u32x2{lo[p], hi[p]};
+      };
+      constexpr std::integral_constant<int, 2> two{};
+      constexpr std::integral_constant<int, OPL> out_pl{};
+      const auto publish_top = [&](float m, float (&t)[16][4]) {
+        m = max_quarters(m);
+        if (lq == 0) t[lr][w] = m;
+      };
+      const auto top_state = [&]() {
+        float ms = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KT; ++i) ms = largest(ms, S[i]);
+        publish_top(16.0f * ms, top_s);
+      };
 
-  while (true) {
-    const int done_next = done + n, done_2 = done_next + n_1;
-    const bool more = done_next < r.n;
-    const int in_2 = after(in_1, n_1), n_2 = done_2 < r.n ? length(done_2, in_2) : 0;
-    const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
-    const float end = end_check[0];
-    const bool check = __builtin_amdgcn_readfirstlane(__float_as_int(end_check[1])) != 0;
-    lds_barrier();
-    // Planes are read before the columns' sizes are looked at, and again where
-    // those call for it. Loads from memory go out while LDS answers: a wave that
-    // waits for their path to take them would otherwise hold the chain up.
-    u32x4 sp[KS][2];
-    const auto read_s = [&]() {
+      load_v(n, vv);
+      if (done == 0)
 #pragma unroll
-      for (int i = OWN; i < KS; ++i)
+        for (int i = 0; i < KT; ++i) {
+          S[i] = f32x4{0, 0, 0, 0};
+          if (!r.fresh && column && 16 * (w * KT + i) + 4 * lq < a.K)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) sp[i][p] = *reinterpret_cast<const u32x4 *>(&Sp[p][0][0] + s_at[i]);
-    };
-    const float m = top(top_s);
-    read_s();
-    asm volatile("" ::: "memory");  // reads stay above the branch
-    load_kt();
-    ktp += kstep;
-    kp += kstep;
-    tp += vstep;
-    sc += vstep;
-    end_check = load_end();
-    {
-      const bool fits = column_fits(m);
-      if (__builtin_amdgcn_ballot_w64(!fits) != 0) {
-        rescale(fits ? 1.0f : kColumnAim * inverse_power(m));
-        publish_s();
+            for (int e = 0; e < 4; ++e) S[i][e] = load_as_f32(a.state, state_at(r.src, i) + e, a.state_dt);
+        }
+      // In the order of the loop: a wait counts the loads behind the one it is for.
+      f32x2 end_check = load_end();
+      load_k();
+      f32x4 in_scale = scalars(kScIn);
+      // The next two chunks' tokens: their lengths are needed as their loads start.
+      int in_1 = after(inside, n), n_1 = done + n < r.n ? length(done + n, in_1) : 0;
+      load_v(n_1, v_next);
+      load_t();
+      f32x4 out_decay = scalars(kScOut);
+      loads_done();
+      top_state();
+      publish_s();
+
+      bool more, check;
+      int done_next, in_2, n_2;
+      float end;
+      u32x4 sp[KS][2];
+      const auto read_s = [&]() {
+#pragma unroll
+        for (int i = OWN; i < KS; ++i)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) sp[i][p] = *reinterpret_cast<const u32x4 *>(&Sp[p][0][0] + s_at[i]);
+      };
+      // A chunk's start: S0 from the other waves, and its size. False where the
+      // chunk is walked. The loop over chunks ends in one place, below: with a way
+      // out up here the compiler moves what is being loaded, and waits for it.
+      const auto enter = [&]() -> bool {
+        done_next = done + n;
+        more = done_next < r.n;
+        in_2 = after(in_1, n_1), n_2 = done_next + n_1 < r.n ? length(done_next + n_1, in_2) : 0;
+        const int64_t kstep = more ? key_step : 0, vstep = more ? value_step : 0;
+        // A register of its own: as end_check's, the load below would take another,
+        // and the loop's end would wait for it to move it back.
+        asm volatile("v_mov_b32 %0, %1" : "=v"(end) : "v"(end_check[0]));
+        check = __builtin_amdgcn_readfirstlane(__float_as_int(end_check[1])) != 0;
         lds_barrier();
+        // Planes are read before the columns' sizes are looked at, and again where
+        // those call for it. Loads from memory go out while LDS answers: a wave that
+        // waits for their path to take them would otherwise hold the chain up.
+        const f32x4 tops = *reinterpret_cast<const f32x4 *>(top_s[lr]);
+        const f32x2 v_tops = *reinterpret_cast<const f32x2 *>(tops_v[lr]);
         read_s();
+        asm volatile("" ::: "memory");  // reads stay above the branch
+        load_kt();
+        ktp += kstep;
+        kp += kstep;
+        tp += vstep;
+        sc += vstep;
+        end_check = load_end();
+        const float state = largest(0.0f, tops), m = fmaxf(state, sigma * v_tops[0]);
+        const uint64_t spans = __builtin_amdgcn_ballot_w64(state <= sigma * v_tops[1]);
+        if (inside_window(m) != ~0ull) {
+          rescale(column_fits(m) ? 1.0f : kColumnAim * inverse_power(m));
+          publish_s();
+          lds_barrier();
+          read_s();
+        }
+        return spans == ~0ull;
+      };
+      bool go = enter();
+      while (go) {
+        // X = K S0^T.
+#pragma unroll
+        for (int i = OWN; i < KS; ++i) {
+          X[0] = mfma(kf[i][0], sp[i][0], X[0]);
+          X[1] = mfma(kf[i][0], sp[i][1], X[1]);
+          if constexpr (PL == 2) X[1] = mfma(kf[i][1], sp[i][0], X[1]);
+        }
+        // R = v - diag(e^G) X.
+        f32x4 R;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) R[i] = fmaf(-in_scale[i], X[0][i] + X[1][i], sigma * value(vv[i]));
+        publish_rows(R, two, &Rp[0][0][0]);
+        if (check) publish_top(largest(0.0f, R), top_r);
+        lds_barrier();
+        if (check) {
+          const float f = back_inside(top(top_r));
+          R *= f;
+          rescale(f);
+          publish_rows(R, two, &Rp[0][0][0]);
+          lds_barrier();
+        }
+        // c = T R, d = diag(e^{G_end - G}) c.
+        f32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        u32x4 rp[2][2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) rp[0][p] = shared(Rp[p][0]);
+        if (low)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) rp[1][p] = shared(Rp[p][1]);
+        load_k();
+        in_scale = scalars(kScIn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("v_mov_b32 %0, %1" : "=v"(vv[i]) : "v"(v_next[i]));  // alike
+        load_v(n_2, v_next);
+        c[0] = mfma(tf[0][0], rp[0][0], c[0]);
+        c[1] = mfma(tf[0][1], rp[0][0], c[1]);
+        c[1] = mfma(tf[0][0], rp[0][1], c[1]);
+        if (low) {
+          c[0] = mfma(tf[1][0], rp[1][0], c[0]);
+          c[1] = mfma(tf[1][1], rp[1][0], c[1]);
+          c[1] = mfma(tf[1][0], rp[1][1], c[1]);
+        }
+        c[0] = (c[0] + c[1]) * kTDown;
+        f32x4 d = c[0] * out_decay;
+        publish_rows(d, two, &Dp[0][0][0]);
+        publish_rows(c[0], out_pl, &Cp[0][0][0]);
+        if (check) publish_top(largest(largest(0.0f, c[0]), d), top_c);
+        lds_barrier();
+        if (check) {
+          const float f = back_inside(top(top_c));
+          rescale(f);
+          publish_rows(d * f, two, &Dp[0][0][0]);
+          publish_rows(c[0] * f, out_pl, &Cp[0][0][0]);
+          lds_barrier();
+        }
+        // S1 = e^{G_end} S0 + K^T d.
+        u32x4 dp[2][2];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) dp[ks][p] = shared(Dp[p][ks]);
+        load_t();
+        out_decay = scalars(kScOut);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] *= end;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][0], S[i]);
+#pragma unroll
+          for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][1], S[i]);
+          if constexpr (PL == 2)
+#pragma unroll
+            for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][1], dp[ks][0], S[i]);
+        }
+        go = false;
+        if (more) {
+          publish_s();
+          top_state();
+          if (a.align && in_1 == 0) {
+            const int64_t page = boundary_page(a.pages, r, r.C + done_next);
+            if (page != 0) store_state(page);
+          }
+          done = done_next;
+          inside = in_1;
+          n = n_1;
+          in_1 = in_2;
+          n_1 = n_2;
+          ++chunk;
+          go = enter();
+        } else {
+          done = r.n;
+        }
       }
-    }
-    // X = K S0^T.
+      if (done == r.n) {
+        store_state(r.fin);
+        return;
+      }
+      // A walked chunk.
+      rescale(unscale);
+      WalkState<KT> state;
 #pragma unroll
-    for (int i = OWN; i < KS; ++i) {
-      X[0] = mfma(kf[i][0], sp[i][0], X[0]);
-      X[1] = mfma(kf[i][0], sp[i][1], X[1]);
-      if constexpr (PL == 2) X[1] = mfma(kf[i][1], sp[i][0], X[1]);
-    }
-    // R = v - diag(e^G) X.
-    f32x4 R;
+      for (int i = 0; i < KT; ++i) state.s[i] = S[i];
+      const void *const args = (const void *)__builtin_amdgcn_kernarg_segment_ptr();  // the launch's only one
+      state = walk_chunk_split<A, Out, KT>(state, args, sums_of, r.bos + done, n, hv, h, v0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) R[i] = fmaf(-in_scale[i], X[0][i] + X[1][i], sigma * value(vv[i]));
-    publish_rows(R, two, &Rp[0][0][0]);
-    if (check) publish_top(largest(0.0f, R), top_r);
-    lds_barrier();
-    if (check) {
-      const float f = back_inside(top(top_r));
-      R *= f;
-      rescale(f);
-      publish_rows(R, two, &Rp[0][0][0]);
-      lds_barrier();
-    }
-    // c = T R, d = diag(e^{G_end - G}) c.
-    f32x4 c[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    u32x4 rp[2][2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) rp[0][p] = shared(Rp[p][0]);
-    if (low)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) rp[1][p] = shared(Rp[p][1]);
-    load_k();
-    in_scale = scalars(kScIn);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vv[i] = v_next[i];
-    load_v(n_2, v_next);
-    c[0] = mfma(tf[0][0], rp[0][0], c[0]);
-    c[1] = mfma(tf[0][1], rp[0][0], c[1]);
-    c[1] = mfma(tf[0][0], rp[0][1], c[1]);
-    if (low) {
-      c[0] = mfma(tf[1][0], rp[1][0], c[0]);
-      c[1] = mfma(tf[1][1], rp[1][0], c[1]);
-      c[1] = mfma(tf[1][0], rp[1][1], c[1]);
-    }
-    c[0] += c[1];
-    f32x4 d = c[0] * out_decay;
-    publish_rows(d, two, &Dp[0][0][0]);
-    publish_rows(c[0], out_pl, &Cp[0][0][0]);
-    if (check) publish_top(largest(largest(0.0f, c[0]), d), top_c);
-    lds_barrier();
-    if (check) {
-      const float f = back_inside(top(top_c));
-      rescale(f);
-      publish_rows(d * f, two, &Dp[0][0][0]);
-      publish_rows(c[0] * f, out_pl, &Cp[0][0][0]);
-      lds_barrier();
-    }
-    // S1 = e^{G_end} S0 + K^T d.
-    u32x4 dp[2][2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) dp[ks][p] = shared(Dp[p][ks]);
-    load_t();
-    out_decay = scalars(kScOut);
-#pragma unroll
-    for (int i = 0; i < KT; ++i) S[i] *= end;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][0], S[i]);
-#pragma unroll
-      for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][0], dp[ks][1], S[i]);
-      if constexpr (PL == 2)
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = mfma(kt[ks][i][1], dp[ks][0], S[i]);
-    }
-    if (!more) break;
-    publish_s();
-    top_state(vv);
-    if (a.align && in_1 == 0) {
-      const int64_t page = boundary_page(a.pages, r, r.C + done_next);
+      for (int i = 0; i < KT; ++i) S[i] = state.s[i];
+      const int64_t page = done + n == r.n ? r.fin
+                           : a.align && after(inside, n) == 0 ? boundary_page(a.pages, r, r.C + done + n)
+                                                              : 0;
       if (page != 0) store_state(page);
     }
-    done = done_next;
-    n = n_1;
-    in_1 = in_2;
-    n_1 = n_2;
+    // Both, behind a walked chunk.
+    done += n;
+    if (done == r.n) return;
+    inside = after(inside, n);
+    n = length(done, inside);
   }
-  store_state(r.fin);
 }
 
 template <typename A, typename Out, int KP, int NW>
@@ -1397,12 +1761,11 @@ static void launch_prefill_dims(int nw, unsigned scan_grid, hipStream_t s, const
     hipLaunchKernelGGL((scan_split_kernel<A, Out, KP>), dim3(scan_grid), dim3(kSplitThreads), 0, s, a);
     return;
   }
-  if constexpr (scan_staged(key_planes<A>(), out_planes<Out>(), KP)) {
-    if (nw == 1) return launch_scan<A, Out, KP, 1>(scan_grid, s, a);
-    if (nw == 2) return launch_scan<A, Out, KP, 2>(scan_grid, s, a);
-    if (nw == 8) return launch_scan<A, Out, KP, 8>(scan_grid, s, a);
-  }
-  launch_scan<A, Out, KP, 4>(scan_grid, s, a);
+  constexpr bool STAGED = scan_staged(key_planes<A>(), out_planes<Out>(), KP);
+  if constexpr (STAGED || key_planes<A>() == 2)
+    if (nw == 4) launch_scan<A, Out, KP, 4>(scan_grid, s, a);
+  if constexpr (STAGED)
+    if (nw == 8) launch_scan<A, Out, KP, 8>(scan_grid, s, a);
 }
 template <typename A, typename Out>
 void launch_prefill(int kp, int nw, unsigned scan_grid, hipStream_t s, const PrefillArgs &a);
