@@ -5,10 +5,12 @@
 //
 // A thread owns CH neighbouring channels over a tile of tokens and walks them
 // with the last taps - 1 inputs in registers, so each input is read once (and
-// taps - 1 of them again at a tile's start). Bound by reading x and writing
-// out. Whoever has a row's first token also writes its states, final and
-// boundary alike, from x: the only thread that reads the source page's
-// channels is the one that overwrites them, whatever pages coincide.
+// taps - 1 of them again at a tile's start). Bound by reading x and writing out;
+// few registers a thread, for many waves, count for more than wide loads (eight
+// channels and eight tokens at once: 95 us where these take 68). Whoever has a row's first token has all tokens that look back into the
+// source page, also those behind its tile, and writes the row's states, final
+// and boundary alike, from x: the only thread that reads a page's channels is
+// the one that overwrites them.
 #include "rows.cuh"
 
 namespace gdn {
@@ -50,18 +52,31 @@ __device__ __forceinline__ void store_live(T *p, int live, const float (&x)[N]) 
   }
 }
 
+// FP32 outputs take the exact exponential and quotient; 16-bit ones the
+// hardware's (a few 2^-24 each, against a rounding of 2^-12 or more), a fifth of
+// the instructions.
+template <typename T>
+__device__ __forceinline__ float silu(float s) {
+  if constexpr (sizeof(T) == 4) return s / (1.0f + expf(-s));
+  else return s * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * -1.4426950408889634f));
+}
+
+constexpr int U = 4;  // tokens whose inputs a thread asks for at once
+
 template <typename T, int TAPS, int CH>
 __global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
-  constexpr int HIST = TAPS - 1, U = 8;
+  constexpr int HIST = TAPS - 1;
   const gdn_row_pages &p = a.pages;
   const int d0 = (int(blockIdx.x % unsigned(a.groups)) * kConvThreads + int(threadIdx.x)) * CH;
   const int live = a.D - d0 < CH ? a.D - d0 : CH;
   int t = int(blockIdx.x / unsigned(a.groups)) * a.tile;
   const int t1 = t + a.tile < p.tokens ? t + a.tile : int(p.tokens);
   // Rows are found by whole waves; lanes past the channels leave after that.
-  int b = last_not_above(int(p.rows) + 1, t, [&](int i) {
-    return load_index(p.query_start_loc, i * p.qsl_stride, p.qsl_dtype);
-  });
+  const auto start = [&](int i) { return load_index(p.query_start_loc, i * p.qsl_stride, p.qsl_dtype); };
+  // Row t first, which it is where every row has one token: a search is a chain
+  // of loads.
+  int b = t;
+  if (t >= p.rows || start(t) > t || start(t + 1) <= t) b = last_not_above(int(p.rows) + 1, t, start);
   b = __builtin_amdgcn_readfirstlane(b);
   if (live <= 0) return;
   float w[CH][TAPS], bias[CH];
@@ -79,9 +94,16 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
   if (b < 0) b = 0;
   for (; t < t1 && b < p.rows; ++b) {
     const Row r = load_row(p, b);
-    const int end = r.bos + r.n < t1 ? r.bos + r.n : t1;
+    int end = r.bos + r.n < t1 ? r.bos + r.n : t1;
     if (r.n == 0 || end <= t) continue;
     t = t < r.bos ? r.bos : t;
+    if (r.valid && t < r.bos + HIST) {
+      // Tokens that look back into the page go with the row's first.
+      const int near = r.n < HIST ? r.bos + r.n : r.bos + HIST;
+      if (t > r.bos) t = near;
+      else if (end < near) end = near;
+      if (end <= t) continue;
+    }
     if (!r.valid) {
       const float zero[CH] = {};
       for (; t < end; ++t) store_live<T, CH>(out + t * a.out_ts, live, zero);
@@ -89,41 +111,56 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
     }
     float h[HIST][CH];  // the inputs before t, oldest first
     T *const states = static_cast<T *>(a.states);
-    const auto from_page = [&](int j, float (&to)[CH]) {
-      const T *s = states + r.src * a.bs + d0 * a.ds + j * a.ts;
+    if (t == r.bos) {
+      const T *s = states + r.src * a.bs + d0 * a.ds;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) to[c] = !r.fresh && c < live ? to_f32(s[c * a.ds]) : 0.0f;
-    };
+      for (int c = 0; c < CH; ++c) {
+        float past[HIST];
 #pragma unroll
-    for (int j = 0; j < HIST; ++j) {
-      const int at = t - r.bos - HIST + j;  // position in the row
-      if (at >= 0)
-        load_live<T, CH>(x + (r.bos + at) * a.x_ts, live, h[j]);
-      else
-        from_page(HIST + at, h[j]);
+        for (int j = 0; j < HIST; ++j) past[j] = 0.0f;
+        if (!r.fresh && c < live) {
+          if (a.ts == 1) load_live<T, HIST>(s + c * a.ds, HIST, past);
+          else
+#pragma unroll
+            for (int j = 0; j < HIST; ++j) past[j] = to_f32(s[c * a.ds + j * a.ts]);
+        }
+#pragma unroll
+        for (int j = 0; j < HIST; ++j) h[j][c] = past[j];
+      }
+    } else {  // at least HIST tokens into the row
+#pragma unroll
+      for (int j = 0; j < HIST; ++j) load_live<T, CH>(x + int64_t(t - HIST + j) * a.x_ts, live, h[j]);
     }
     if (t == r.bos) {
       // The states: the HIST inputs that end at position pos of the row, taken
       // from the page's history (h, at this point) where pos < HIST.
       const auto store_state = [&](int64_t page, int pos) {
+        float in[HIST][CH];
 #pragma unroll
         for (int j = 0; j < HIST; ++j) {
           const int at = pos - HIST + j;
-          float in[CH];
           if (at >= 0) {
-            load_live<T, CH>(x + (r.bos + at) * a.x_ts, live, in);
+            load_live<T, CH>(x + (r.bos + at) * a.x_ts, live, in[j]);
           } else {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-              in[c] = 0.0f;
+              in[j][c] = 0.0f;
 #pragma unroll
-              for (int i = 0; i < HIST; ++i) in[c] = at + HIST == i ? h[i][c] : in[c];
+              for (int i = 0; i < HIST; ++i) in[j][c] = at + HIST == i ? h[i][c] : in[j][c];
             }
           }
-          T *s = states + page * a.bs + d0 * a.ds + j * a.ts;
+        }
+        T *s = states + page * a.bs + d0 * a.ds;
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
-            if (c < live) s[c * a.ds] = from_f32<T>(in[c]);
+        for (int c = 0; c < CH; ++c) {
+          float past[HIST];
+#pragma unroll
+          for (int j = 0; j < HIST; ++j) past[j] = in[j][c];
+          if (c >= live) continue;
+          if (a.ts == 1) store_live<T, HIST>(s + c * a.ds, HIST, past);
+          else
+#pragma unroll
+            for (int j = 0; j < HIST; ++j) s[c * a.ds + j * a.ts] = from_f32<T>(past[j]);
         }
       };
       if (p.block_table) {
@@ -150,7 +187,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
 #pragma unroll
           for (int j = 0; j < HIST; ++j) s = fmaf(w[c][j], h[j][c], s);
           s = fmaf(w[c][HIST], in[u][c], s);
-          y[c] = a.silu ? s / (1.0f + expf(-s)) : s;
+          y[c] = a.silu ? silu<T>(s) : s;
 #pragma unroll
           for (int j = 0; j + 1 < HIST; ++j) h[j][c] = h[j + 1][c];
           h[HIST - 1][c] = in[u][c];
@@ -162,19 +199,40 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(const ConvArgs a) {
   }
 }
 
-template <typename T, int CH>
+// Channels of a thread, by the tokens of its tile (see conv_tile).
+constexpr int conv_channels(int tile) { return tile < 16 ? 2 : 4; }
+
+template <typename T, int TAPS>
+static void launch_conv_taps(dim3 grid, hipStream_t s, const ConvArgs &a) {
+  if (a.tile < 16) hipLaunchKernelGGL((conv_kernel<T, TAPS, conv_channels(1)>), grid, dim3(kConvThreads), 0, s, a);
+  else hipLaunchKernelGGL((conv_kernel<T, TAPS, conv_channels(16)>), grid, dim3(kConvThreads), 0, s, a);
+}
+template <typename T>
 static void launch_conv(int taps, dim3 grid, hipStream_t s, const ConvArgs &a) {
   switch (taps) {
-    case 2: hipLaunchKernelGGL((conv_kernel<T, 2, CH>), grid, dim3(kConvThreads), 0, s, a); break;
-    case 3: hipLaunchKernelGGL((conv_kernel<T, 3, CH>), grid, dim3(kConvThreads), 0, s, a); break;
-    case 4: hipLaunchKernelGGL((conv_kernel<T, 4, CH>), grid, dim3(kConvThreads), 0, s, a); break;
-    default: hipLaunchKernelGGL((conv_kernel<T, 5, CH>), grid, dim3(kConvThreads), 0, s, a); break;
+    case 2: launch_conv_taps<T, 2>(grid, s, a); break;
+    case 3: launch_conv_taps<T, 3>(grid, s, a); break;
+    case 4: launch_conv_taps<T, 4>(grid, s, a); break;
+    default: launch_conv_taps<T, 5>(grid, s, a); break;
   }
 }
 
 }  // namespace gdn
 
 using namespace gdn;
+
+// Tokens of a thread's tile: 16 of four channels where rows are long and there
+// are threads enough, for fewer inputs read twice; one where every row has one,
+// whose rows a longer tile would take one after the other; else four of two
+// channels. BF16, 4 taps, 8192 channels, us at 1 / 4 / 16 tokens: 256 rows of 1
+// 18.5 / 18.2 / 58, of 2 35 / 22 / 41, of 8 84 / 42 / 38, of 32 361 / 162 / 117;
+// 32 rows of 16 21 / 12 / 13; one row of 512 20 / 10 / 12; 6 rows of 1, 1024
+// channels 4.0 / 9.1 / 20. 8191 tokens in 24 rows: 68 us, 270 MB read and written
+// at 4.0 TB/s.
+static int conv_tile(int64_t tokens, int64_t rows, int64_t dim) {
+  if (tokens <= rows) return 1;
+  return tokens * dim >= (1 << 24) && tokens >= 8 * rows ? 16 : 4;
+}
 
 extern "C" int gdn_recoverssm_conv(const gdn_conv_rows *l, void *stream) {
   int status = GDN_OK;
@@ -200,10 +258,9 @@ extern "C" int gdn_recoverssm_conv(const gdn_conv_rows *l, void *stream) {
   a.x_ts = l->x_stride, a.out_ts = l->out_stride;
   a.bs = l->state_block_stride, a.ds = l->state_dim_stride, a.ts = l->state_token_stride;
   a.D = int32_t(l->dim), a.silu = l->silu;
-  const bool wide = l->pages.tokens >= 8 * l->pages.rows;
-  a.tile = wide ? 32 : 1;
-  const int ch = wide ? 8 : 2;
-  a.groups = int32_t((l->dim + kConvThreads * ch - 1) / (kConvThreads * ch));
+  a.tile = conv_tile(l->pages.tokens, l->pages.rows, l->dim);
+  const int per = kConvThreads * conv_channels(a.tile);
+  a.groups = int32_t((l->dim + per - 1) / per);
   const int64_t blocks = (l->pages.tokens + a.tile - 1) / a.tile * a.groups;
   if (blocks > 0x7fffffffLL) {
     set_error("conv: grid too large");
@@ -211,15 +268,9 @@ extern "C" int gdn_recoverssm_conv(const gdn_conv_rows *l, void *stream) {
   }
   const dim3 grid = dim3(unsigned(blocks));
   auto s = static_cast<hipStream_t>(stream);
-  if (wide) {
-    if (l->dtype == GDN_DT_BF16) launch_conv<bf16, 8>(int(l->taps), grid, s, a);
-    else if (l->dtype == GDN_DT_F16) launch_conv<f16, 8>(int(l->taps), grid, s, a);
-    else launch_conv<float, 8>(int(l->taps), grid, s, a);
-  } else {
-    if (l->dtype == GDN_DT_BF16) launch_conv<bf16, 2>(int(l->taps), grid, s, a);
-    else if (l->dtype == GDN_DT_F16) launch_conv<f16, 2>(int(l->taps), grid, s, a);
-    else launch_conv<float, 2>(int(l->taps), grid, s, a);
-  }
+  if (l->dtype == GDN_DT_BF16) launch_conv<bf16>(int(l->taps), grid, s, a);
+  else if (l->dtype == GDN_DT_F16) launch_conv<f16>(int(l->taps), grid, s, a);
+  else launch_conv<float>(int(l->taps), grid, s, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) {
     set_error("conv: launch failed: %s", hipGetErrorString(err));

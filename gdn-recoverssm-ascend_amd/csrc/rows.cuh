@@ -111,7 +111,7 @@ inline bool index_type(int32_t dt) { return dt == GDN_DT_I32 || dt == GDN_DT_I64
 inline int64_t type_bytes(int32_t dt) { return dt == GDN_DT_F32 ? 4 : 2; }
 
 // Gates of one token and head as the rule takes them: log decay and beta,
-// from the raw projections when the gating is fused (vLLM's fused_gdn_gating).
+// from the raw projections when the gating is fused.
 struct GateParams {
   float neg_exp_a, dt_bias, softplus_beta, softplus_threshold;
   bool gated;
