@@ -368,7 +368,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The same stream as torch.cuda.current_stream's, without its wrapper object (1.5 us a call).
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def i64_array(values) -> ctypes.Array:

@@ -61,7 +61,9 @@ _ROW_RULES = (
     ("the block table must be two-dimensional with at least one column",
      lambda p: p[4] is None or (p[4].ndim == 2 and p[4].shape[1] > 0)),
     ("offsets, indices, lengths and the block table must be int32 or int64",
-     lambda p: all(t is None or t.dtype in _INDEX_TYPES for t in p[:6])),
+     lambda p: p[0].dtype in _INDEX_TYPES and p[1].dtype in _INDEX_TYPES
+     and (p[2] is None or p[2].dtype in _INDEX_TYPES) and (p[3] is None or p[3].dtype in _INDEX_TYPES)
+     and (p[4] is None or p[4].dtype in _INDEX_TYPES) and (p[5] is None or p[5].dtype in _INDEX_TYPES)),
 )
 
 
@@ -70,8 +72,9 @@ def _row_pages(parts: tuple, tokens: int, blocks: int, device) -> N.RowPages:
     (query_start_loc, state_indices, final_indices, num_computed, block_table,
     request_indices, block_size)."""
     enforce(_ROW_RULES, parts)
-    if any(t is not None and t.device != device for t in parts[:6]):
-        fail("inputs must be on the same device")
+    for t in parts[:6]:
+        if t is not None and t.device != device:
+            fail("inputs must be on the same device")
     qsl, source, final, computed, table, requests, block = parts
     p = N.RowPages(qsl.data_ptr(), source.data_ptr())
     p.rows, p.tokens, p.blocks = source.shape[0], tokens, blocks
@@ -93,37 +96,41 @@ def _row_pages(parts: tuple, tokens: int, blocks: int, device) -> N.RowPages:
 
 
 _RULE_RULES = (
-    ("q must have shape [1, tokens, heads, dim]", lambda c: c.q.ndim == 4 and c.q.shape[0] == 1),
-    ("q and k shapes differ", lambda c: c.k.shape == c.q.shape),
+    ("q must have shape [1, tokens, heads, dim]", lambda c: len(c.qs) == 4 and c.qs[0] == 1),
+    ("q and k shapes differ", lambda c: c.k.shape == c.qs),
     ("v must have shape [1, tokens, value heads, dim]",
-     lambda c: c.v.ndim == 4 and c.v.shape[0] == 1 and c.v.shape[1] == c.q.shape[1]),
+     lambda c: len(c.vs) == 4 and c.vs[0] == 1 and c.vs[1] == c.qs[1]),
     ("value heads must be a positive multiple of the q/k heads",
-     lambda c: 0 < c.q.shape[2] <= c.v.shape[2] and c.v.shape[2] % c.q.shape[2] == 0),
+     lambda c: 0 < c.qs[2] <= c.vs[2] and c.vs[2] % c.qs[2] == 0),
     ("q, k and v heads must be contiguous",
-     lambda c: all(t.stride(3) == 1 and t.stride(2) == t.shape[3] for t in (c.q, c.k, c.v))),
+     lambda c: c.q.stride()[2:] == (c.qs[3], 1) and c.k.stride()[2:] == (c.qs[3], 1)
+     and c.v.stride()[2:] == (c.vs[3], 1)),
     ("q, k and v must share one activation dtype (FP32, BF16 or FP16)",
-     lambda c: c.q.dtype == c.k.dtype == c.v.dtype and c.q.dtype in _FLOAT_TYPES),
-    ("gate or beta shape is incompatible", lambda c: all(t.numel() == c.v.shape[1] * c.v.shape[2] for t in (c.g, c.beta))),
+     lambda c: c.act == c.k.dtype == c.v.dtype and c.act in _FLOAT_TYPES),
+    ("gate or beta shape is incompatible",
+     lambda c: c.g.numel() == c.vs[1] * c.vs[2] and c.beta.numel() == c.vs[1] * c.vs[2]),
     ("gate and beta must be FP32 or the activation dtype",
-     lambda c: all(t.dtype in (torch.float32, c.q.dtype) for t in (c.g, c.beta))),
-    ("checkpoint must be four-dimensional", lambda c: c.state.ndim == 4),
+     lambda c: c.g.dtype in (torch.float32, c.act) and c.beta.dtype in (torch.float32, c.act)),
+    ("checkpoint must be four-dimensional", lambda c: len(c.ss) == 4),
     ("checkpoint shape is incompatible",
-     lambda c: tuple(c.state.shape[1:]) == (c.v.shape[2], c.v.shape[3], c.q.shape[3]) and c.state.shape[0] > 0),
+     lambda c: c.ss[1:] == (c.vs[2], c.vs[3], c.qs[3]) and c.ss[0] > 0),
     ("checkpoint dtype is not supported", lambda c: c.state.dtype in _FLOAT_TYPES),
     (f"checkpoint rows must be contiguous, 16-byte aligned and K <= {MAX_KEY_DIM} a multiple of 16 bytes",
-     lambda c: c.q.shape[3] <= MAX_KEY_DIM and c.state.stride(3) == 1 and c.state.data_ptr() % 16 == 0
-     and all(s * c.state.element_size() % 16 == 0 for s in (c.q.shape[3], *c.state.stride()[:3]))),
+     lambda c: c.qs[3] <= MAX_KEY_DIM and c.strides[3] == 1 and c.state.data_ptr() % 16 == 0
+     # 16 bytes of elements divide the dim and every stride
+     and not (c.qs[3] | c.strides[0] | c.strides[1] | c.strides[2]) % (16 // c.state.element_size())),
     ("output shape or layout is incompatible",
-     lambda c: c.out.shape == c.v.shape and c.out.stride(3) == 1 and c.out.stride(2) == c.v.shape[3]),
-    ("out must be FP32 or the activation dtype", lambda c: c.out.dtype in (torch.float32, c.q.dtype)),
+     lambda c: c.out.shape == c.vs and c.out.stride()[2:] == (c.vs[3], 1)),
+    ("out must be FP32 or the activation dtype", lambda c: c.out.dtype in (torch.float32, c.act)),
     ("A_log and dt_bias need one contiguous entry per value head",
-     lambda c: c.a_log is None or all(t.ndim == 1 and t.shape[0] == c.v.shape[2] and t.stride(0) == 1
+     lambda c: c.a_log is None or all(t.ndim == 1 and t.shape[0] == c.vs[2] and t.stride(0) == 1
                                       and t.dtype in _FLOAT_TYPES for t in (c.a_log, c.dt_bias))),
     ("softplus beta must be positive", lambda c: c.a_log is None or c.softplus[0] > 0.0),
     ("inputs must be on the same device",
-     lambda c: all(t is None or t.device == c.q.device
-                   for t in (c.k, c.v, c.g, c.beta, c.state, c.out, c.a_log, c.dt_bias))),
-    ("prefill and decode run on a HIP device", lambda c: c.q.device.type == "cuda"),
+     lambda c: c.k.device == c.device and c.v.device == c.device and c.g.device == c.device
+     and c.beta.device == c.device and c.state.device == c.device and c.out.device == c.device
+     and (c.a_log is None or (c.a_log.device == c.device and c.dt_bias.device == c.device))),
+    ("prefill and decode run on a HIP device", lambda c: c.device.type == "cuda"),
 )
 
 
@@ -132,25 +139,27 @@ class _RuleCall:
 
     def __init__(self, g, beta, q, k, v, state, out, a_log=None, dt_bias=None, softplus=(1.0, 20.0)):
         self.g, self.beta, self.q, self.k, self.v, self.state = g, beta, q, k, v, state
-        self.out = torch.empty(v.shape, dtype=v.dtype, device=v.device) if out is None else out
+        self.qs, self.vs, self.ss, self.strides = q.shape, v.shape, state.shape, state.stride()
+        self.act, self.device = q.dtype, q.device
+        self.out = torch.empty(self.vs, dtype=v.dtype, device=v.device) if out is None else out
         self.a_log, self.dt_bias, self.softplus = a_log, dt_bias, softplus
 
     def launch(self, parts, scale, normalized) -> N.RuleLaunch:
         enforce(_RULE_RULES, self)
         q, k, v, state, out = self.q, self.k, self.v, self.state, self.out
-        tokens, heads, K = q.shape[1:]
-        HV, V = v.shape[2:]
+        _, tokens, heads, K = self.qs
+        _, _, HV, V = self.vs
         g, beta = self.g.reshape(tokens, HV), self.beta.reshape(tokens, HV)
         if HV > 1 and (g.stride(1) != 1 or beta.stride(1) != 1):
             fail("gate and beta heads must be contiguous")
-        pages = _row_pages(parts, tokens, state.shape[0], q.device)
+        pages = _row_pages(parts, tokens, self.ss[0], self.device)
         gating = a_log = dt_bias = None
         if self.a_log is not None:
             a_log, dt_bias = self.a_log.data_ptr(), self.dt_bias.data_ptr()
             self.gating = N.GatingExt(N.dtype_code(self.a_log.dtype), N.dtype_code(self.dt_bias.dtype), *self.softplus)
             gating = ctypes.pointer(self.gating)
         self.keep = (g, beta)  # what the pointers below name
-        strides = state.stride()
+        strides = self.strides
         return N.RuleLaunch(
             pages, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
             state.data_ptr(), a_log, dt_bias, gating, heads, HV, K, V, q.stride(1), k.stride(1), v.stride(1),
@@ -165,14 +174,14 @@ class _RuleCall:
         nbytes = lib.gdn_recoverssm_prefill_workspace(ref)
         if nbytes < 0:
             N.check(N.GDN_ERR_UNSUPPORTED, "prefill")
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.q.device) if nbytes else None
-        N.check(lib.gdn_recoverssm_prefill(ref, N.ptr(workspace), nbytes, N.stream_handle(self.q.device)), "prefill")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        N.check(lib.gdn_recoverssm_prefill(ref, N.ptr(workspace), nbytes, N.stream_handle(self.device)), "prefill")
         _COUNTS["prefill"] += 1
         return self.out
 
     def decode(self, parts, scale, normalized):
         launch = self.launch(parts, scale, normalized)
-        N.check(N.load().gdn_recoverssm_decode(ctypes.byref(launch), N.stream_handle(self.q.device)), "decode")
+        N.check(N.load().gdn_recoverssm_decode(ctypes.byref(launch), N.stream_handle(self.device)), "decode")
         _COUNTS["decode"] += 1
         return self.out
 
@@ -316,8 +325,8 @@ MAX_CONV_TAPS = 5
 _CONV_RULES = (
     ("x must have shape [tokens, channels]", lambda x, w, b, s, o: x.ndim == 2 and x.shape[1] > 0),
     ("conv activations, weight, bias, output and states must share one dtype (FP32, BF16 or FP16)",
-     lambda x, w, b, s, o: x.dtype in _FLOAT_TYPES
-     and all(t is None or t.dtype == x.dtype for t in (w, b, s, o))),
+     lambda x, w, b, s, o: x.dtype in _FLOAT_TYPES and x.dtype == w.dtype == s.dtype == o.dtype
+     and (b is None or b.dtype == x.dtype)),
     (f"weight must be contiguous [channels, taps] with 2 to {MAX_CONV_TAPS} taps",
      lambda x, w, b, s, o: w.ndim == 2 and w.shape[0] == x.shape[1] and 2 <= w.shape[1] <= MAX_CONV_TAPS
      and w.is_contiguous()),
@@ -330,7 +339,7 @@ _CONV_RULES = (
     ("output shape or layout is incompatible",
      lambda x, w, b, s, o: o.shape == x.shape and (o.stride(1) == 1 or o.shape[1] == 1)),
     ("inputs must be on the same device",
-     lambda x, w, b, s, o: all(t is None or t.device == x.device for t in (w, b, s, o))),
+     lambda x, w, b, s, o: x.device == w.device == s.device == o.device and (b is None or b.device == x.device)),
     ("the convolution runs on a HIP device", lambda x, w, b, s, o: x.device.type == "cuda"),
 )
 

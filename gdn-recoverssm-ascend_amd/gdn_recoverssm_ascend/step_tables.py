@@ -42,7 +42,8 @@ class StepTables:
         # Two allocations: eight small tensors would cost more host time than the kernel takes.
         words = torch.empty(5 * rows + 1, dtype=torch.int32, device=device)
         longs = torch.empty(2 * num_tokens + 2, dtype=torch.int64, device=device)
-        return cls(*words.split((rows + 1, rows, rows, rows, rows)), *longs.split((num_tokens, num_tokens, 2)))
+        return cls(*words.split_with_sizes((rows + 1, rows, rows, rows, rows)),
+                   *longs.split_with_sizes((num_tokens, num_tokens, 2)))
 
 
 _TABLE_RULES = (
@@ -52,7 +53,8 @@ _TABLE_RULES = (
     ("num_computed needs one entry per row when there are no request_indices",
      lambda c: c.requests is not None or c.computed.shape[0] >= c.lens.shape[0]),
     ("lengths and request indices must be int32 or int64",
-     lambda c: all(t is None or t.dtype in _INDEX_TYPES for t in (c.computed, c.lens, c.requests))),
+     lambda c: c.computed.dtype in _INDEX_TYPES and c.lens.dtype in _INDEX_TYPES
+     and (c.requests is None or c.requests.dtype in _INDEX_TYPES)),
     (f"a call takes at most {MAX_TABLE_ROWS} rows", lambda c: c.lens.shape[0] <= MAX_TABLE_ROWS),
     ("num_tokens must be >= 0", lambda c: c.num_tokens >= 0),
     ("the tables run on a HIP device", lambda c: c.table.device.type == "cuda"),
@@ -116,8 +118,9 @@ def gdn_recoverssm_step_tables(
     enforce(_TABLE_RULES, c)
     enforce(_POOL_RULES, block_table, free_pages, free_span, block_size)
     rows, device = query_lens.shape[0], block_table.device
-    if any(t is not None and t.device != device for t in (num_computed, query_lens, request_indices)):
-        fail("inputs must be on the same device")
+    for t in (num_computed, query_lens, request_indices):
+        if t is not None and t.device != device:
+            fail("inputs must be on the same device")
     if out is None:
         out = StepTables.allocate(rows, c.num_tokens, device)
     else:
