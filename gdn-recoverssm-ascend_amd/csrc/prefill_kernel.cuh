@@ -16,17 +16,26 @@
 // matrix cores with an FP32 operand as the sum of two F16 planes of 11 bits (its
 // rounding to F16, and that of what the rounding left: 2^-23 of a value). F16
 // has no FP32's range, so every operand is scaled by powers of two, which cost
-// no bits: rows of K and Q by their largest element, T by nothing (|T| <= 2
-// where the rule is stable), and all that is linear in a column of V (S0, v, c,
-// out) by one factor a column that the scan follows from chunk to chunk. A
-// product of two split operands drops the two low planes' product, 2^-24 of it.
-// Outputs rounded to BF16 take one plane of S0, P and c (2^-12); F16 and FP32
-// ones two. Three BF16 planes need no scaling and were tried first: 1.5 times
-// the products and planes, and twice the instructions that make them. The FP32
-// matrix instruction takes 16 times an F16 one's time.
+// no bits: rows of K and Q by their largest element, and all that is linear in a
+// column of V (S0, v, c, out) by one factor a column that the scan follows from
+// chunk to chunk. With K = diag(m) K' the kernels hold c' = diag(m) c in c's
+// place, so m stands beside beta in T and L and nowhere else; with the L2 norm
+// fused in, m and Q's factor take 1 / |k| and 1 / |q|. A product of two split
+// operands drops the two low planes' product, 2^-24 of it. Outputs rounded to
+// BF16 take one plane of S0, P and c (2^-12); F16 and FP32 ones two. Three BF16
+// planes need no scaling and were tried first: 1.5 times the products and planes,
+// and twice the instructions that make them (the scan of 8 Ki tokens took 818 us
+// in its first form, 266 us at its best). The FP32 matrix instruction takes 16
+// times an F16 one's time. An error is thus 2^-22 of the values it stems from, and
+// at least 2^-25 to 2^-32 of the largest in its column and chunk; columns and
+// chunks for which that is too coarse are walked token by token.
 //
-// With the L2 norm fused in, 1 / |k| and 1 / |q| go into the scalars beside T,
-// P and the decays, and K and Q stay as they are.
+// What bounds it: a row's chunks follow one another, and a chunk is four
+// products each of which needs the one before. 8 Ki tokens of 16 key and 32
+// value heads, K = V = 128, BF16: prepare 77 us, scan 205 us (128 chunks of 1.6
+// us), where the inputs and outputs take 45 us at a copy's rate and the products
+// 23 us at a large matrix product's. Folding T into K^T and P beforehand (two
+// products a chunk, and 32 KB more of operands) made that scan 239 us.
 #pragma once
 
 #include <type_traits>
@@ -237,8 +246,11 @@ __device__ __forceinline__ double wave_prefix(double x) {
 // products K K^T and Q K^T, and T, P and the scalars of each of its value heads.
 // A team of four waves takes a value head, wave w token rows 16w .. 16w + 15;
 // with two teams one loads K and the other Q, and each takes every second value
-// head. Bound by vector instructions: most of a wave's go into converting K and
-// Q and into L and P.
+// head. Of 77 us for 8 Ki tokens (see the top) 40 go into the 188 MB of planes it
+// writes, which all workgroups of a round do together; between its barriers the
+// vector units are a third busy and the matrix units a tenth, two workgroups of
+// eight waves on a compute unit. One workgroup a value head took 146 us (K and Q
+// converted twice); asking for the gates before K and Q, 82 us.
 // ---------------------------------------------------------------------------
 constexpr int prepare_waves(int pl, int kp) { return pl == 1 && kp <= 128 ? 4 : pl == 1 || kp <= 128 ? 2 : 1; }
 
@@ -259,7 +271,8 @@ __device__ __forceinline__ void load_row8(const A *row, bool live, int k0, int K
 }
 
 template <typename A, typename Out, int KP, int TEAMS>
-__global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) void prepare_kernel(const PrefillArgs a) {
+__global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) void prepare_kernel(
+    const PrefillArgs a) {
   using U = Units<A, Out, KP>;
   constexpr int PL = U::PL, OPL = U::OPL, KS = KP / 32, LD = kChunk + 4;
   // Planes of K and Q, then, in their place, a matrix of a value head per team.
@@ -592,7 +605,10 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
 // products of a chunk keep a column of V in one lane group, so a wave needs
 // nothing of another's. NW waves of one head share a workgroup for the sake of
 // what they read: operands go from memory to LDS once for all of them, a chunk
-// ahead (two buffers), without passing registers.
+// ahead (two buffers), without passing registers. 7777 packed tokens of 24 rows,
+// 32 value heads, K = V = 128, BF16, blocks of 256: 147 us, matrix units 18%
+// busy, vector units 29%: a wave's products wait for its own last ones, and two
+// waves a SIMD are what their registers leave room for.
 // ---------------------------------------------------------------------------
 // Byte offsets of a chunk's tokens stay under kScanExtent (the host checks the
 // strides), the size of every resource here. A lane outside the tensor takes
@@ -677,7 +693,8 @@ struct WalkSums {
 // A chunk's tokens one after the other, from the inputs themselves: the state
 // (as it is, unscaled) and the outputs of this wave's 16 columns, lanes as in
 // scan_kernel. Not inlined, so that the loops around the call keep their
-// registers; the launch's arguments are read where they were passed.
+// registers; the launch's arguments are read where they were passed. A token takes
+// 1.8 us, 70 times its share of a chunk: loads from memory one after the other.
 template <int N>
 struct WalkState {
   f32x4 s[N];
@@ -1174,7 +1191,11 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
 // a row's chunks one after the other are all the time there is: a chunk is a
 // quarter of the instructions, for three exchanges through LDS. Operands go from
 // memory into the registers of the one wave that uses them, a chunk ahead: they
-// are refilled as soon as their product has taken them.
+// are refilled as soon as their product has taken them. 1.6 us a chunk at K = 128
+// (8 Ki tokens 205 us; a row of 4 Ki with 4 value heads, 32 workgroups on the
+// whole card, 1.3 us a chunk and 83 us), of which the matrix units work 12%
+// and the 66 KB of operands take half on their way from the L2 to registers; one
+// wave doing all of a column tile's products took 2.6 us.
 // ---------------------------------------------------------------------------
 constexpr int kSplitThreads = 512;
 constexpr int split_waves(int pl, int kp) { return pl == 1 && kp <= 64 ? 4 : 2; }

@@ -216,11 +216,16 @@ def gdn_recoverssm_prefill(
     allocated when not given. States are computed to FP32 precision whatever the
     activation dtype, and rounded once where a page of fewer bits is written. A
     NaN or an infinity among a token's inputs can reach the outputs of up to 63
-    tokens before it in its own row (the chunk), besides those after it.
+    tokens before it in its own row (the chunk), besides those after it. Chunks
+    whose values a matrix core's operands cannot hold (decays that grow, keys far
+    from unit length, columns that fall by a factor of 2^16 within 64 tokens) are
+    computed token by token, some 70 times as slowly.
 
-    Working memory is taken from torch's allocator: 40 KiB per 64 tokens and
-    value head of 16-bit activations, and 16 KiB per 64 tokens and key head at
-    K = 128.
+    Token strides of ``v`` and ``out`` must be at least the value dim and span
+    under 1 GiB per 64 tokens. Working memory is taken from torch's allocator:
+    per 64 tokens 20 KiB a value head (26 KiB where the output is not BF16) and
+    48 KiB a key head at K = 128 (twice that for FP32 activations; K counts as
+    64, 128 or 256).
     """
     return _RuleCall(g, beta, q, k, v, checkpoint_state, out).prefill(
         (query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices, block_size),
