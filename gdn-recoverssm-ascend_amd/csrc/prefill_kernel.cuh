@@ -246,11 +246,12 @@ __device__ __forceinline__ double wave_prefix(double x) {
 // products K K^T and Q K^T, and T, P and the scalars of each of its value heads.
 // A team of four waves takes a value head, wave w token rows 16w .. 16w + 15;
 // with two teams one loads K and the other Q, and each takes every second value
-// head. Of 77 us for 8 Ki tokens (see the top) 40 go into the 188 MB of planes it
-// writes, which all workgroups of a round do together; between its barriers the
-// vector units are a third busy and the matrix units a tenth, two workgroups of
-// eight waves on a compute unit. One workgroup a value head took 146 us (K and Q
-// converted twice); asking for the gates before K and Q, 82 us.
+// head. 8 Ki tokens (see the top) take 77 us, of which the 188 MB of planes it
+// writes would take 40 at a copy's rate; the vector units are a third busy, the
+// matrix units a tenth: two workgroups of eight waves on a compute unit do not
+// hide each other's barriers and round trips. One team taking the value heads in
+// turn took 94 us where two took 85; asking for the gates before K and Q 82 us
+// where this takes 77.
 // ---------------------------------------------------------------------------
 constexpr int prepare_waves(int pl, int kp) { return pl == 1 && kp <= 128 ? 4 : pl == 1 || kp <= 128 ? 2 : 1; }
 
