@@ -38,6 +38,7 @@ RecoverSSM: ...")``); launches go on the current stream without synchronising.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -67,29 +68,46 @@ _ROW_RULES = (
 )
 
 
+# A call checks itself in one expression that only a call keeping every rule
+# satisfies; the rules are gone through, in their order, where it does not (a rule
+# at a time they take twice as long, a quarter of a small call's host time).
+
+
+def _plain_rows(qsl, source, final, computed, requests, device) -> bool:
+    rows = source.shape
+    return (len(rows) == 1 and qsl.shape == (rows[0] + 1,) and qsl.dtype in _INDEX_TYPES
+            and source.dtype in _INDEX_TYPES and qsl.device == device and source.device == device
+            and (final is None or (final.shape == rows and final.dtype in _INDEX_TYPES and final.device == device))
+            and (requests is None or (requests.shape == rows and requests.dtype in _INDEX_TYPES
+                                      and requests.device == device))
+            and (computed is None or (computed.ndim == 1 and computed.dtype in _INDEX_TYPES
+                                      and computed.device == device
+                                      and (requests is not None or computed.shape[0] >= rows[0]))))
+
+
 def _row_pages(parts: tuple, tokens: int, blocks: int, device) -> N.RowPages:
     """The rows' description, checked, as the C ABI takes it; ``parts`` are
     (query_start_loc, state_indices, final_indices, num_computed, block_table,
     request_indices, block_size)."""
-    enforce(_ROW_RULES, parts)
-    for t in parts[:6]:
-        if t is not None and t.device != device:
-            fail("inputs must be on the same device")
     qsl, source, final, computed, table, requests, block = parts
-    p = N.RowPages(qsl.data_ptr(), source.data_ptr())
-    p.rows, p.tokens, p.blocks = source.shape[0], tokens, blocks
-    p.qsl_stride, p.qsl_dtype = qsl.stride(0), N.dtype_code(qsl.dtype)
-    p.si_stride, p.si_dtype = source.stride(0), N.dtype_code(source.dtype)
+    if not (table is None and block is None and _plain_rows(qsl, source, final, computed, requests, device)):
+        enforce(_ROW_RULES, parts)
+        for t in parts[:6]:
+            if t is not None and t.device != device:
+                fail("inputs must be on the same device")
+    code = N.dtype_code
+    p = N.RowPages(qsl.data_ptr(), source.data_ptr(), None, None, None, None, source.shape[0], tokens, blocks,
+                   qsl.stride(0), source.stride(0))
+    p.qsl_dtype, p.si_dtype = code(qsl.dtype), code(source.dtype)
     if final is not None:
-        p.final_indices, p.final_stride, p.final_dtype = final.data_ptr(), final.stride(0), N.dtype_code(final.dtype)
+        p.final_indices, p.final_stride, p.final_dtype = final.data_ptr(), final.stride(0), code(final.dtype)
     if computed is not None:
         p.num_computed, p.computed_len = computed.data_ptr(), computed.shape[0]
-        p.computed_stride, p.computed_dtype = computed.stride(0), N.dtype_code(computed.dtype)
+        p.computed_stride, p.computed_dtype = computed.stride(0), code(computed.dtype)
     if requests is not None:
-        p.request_indices, p.map_stride = requests.data_ptr(), requests.stride(0)
-        p.map_dtype = N.dtype_code(requests.dtype)
+        p.request_indices, p.map_stride, p.map_dtype = requests.data_ptr(), requests.stride(0), code(requests.dtype)
     if table is not None:
-        p.block_table, p.table_dtype, p.block_size = table.data_ptr(), N.dtype_code(table.dtype), block
+        p.block_table, p.table_dtype, p.block_size = table.data_ptr(), code(table.dtype), block
         p.table_rows, p.table_width = table.shape
         p.table_row_stride, p.table_col_stride = table.stride()
     return p
@@ -134,6 +152,12 @@ _RULE_RULES = (
 )
 
 
+@functools.lru_cache(maxsize=64)
+def _gating_ext(a_log_dtype, dt_bias_dtype, softplus_beta, softplus_threshold):
+    return ctypes.pointer(N.GatingExt(N.dtype_code(a_log_dtype), N.dtype_code(dt_bias_dtype), softplus_beta,
+                                      softplus_threshold))
+
+
 class _RuleCall:
     """One call of the rule: its tensors, and the launch that follows."""
 
@@ -141,31 +165,68 @@ class _RuleCall:
         self.g, self.beta, self.q, self.k, self.v, self.state = g, beta, q, k, v, state
         self.qs, self.vs, self.ss, self.strides = q.shape, v.shape, state.shape, state.stride()
         self.act, self.device = q.dtype, q.device
-        self.out = torch.empty(self.vs, dtype=v.dtype, device=v.device) if out is None else out
+        self.out = v.new_empty(self.vs) if out is None else out
         self.a_log, self.dt_bias, self.softplus = a_log, dt_bias, softplus
 
+    def keeps_the_rules(self) -> bool:
+        q, k, v, g, beta, state, out = self.q, self.k, self.v, self.g, self.beta, self.state, self.out
+        qs, vs, act, device, strides = self.qs, self.vs, self.act, self.device, self.strides
+        if not (len(qs) == 4 and len(vs) == 4 and len(strides) == 4):
+            return False
+        one, tokens, heads, K = qs
+        _, _, HV, V = vs
+        g_dtype, beta_dtype, f32 = g.dtype, beta.dtype, torch.float32
+        return (one == 1 and k.shape == qs and vs[0] == 1 and vs[1] == tokens and 0 < heads <= HV and HV % heads == 0
+                and q.stride()[2:] == k.stride()[2:] == (K, 1) and v.stride()[2:] == (V, 1)
+                and act == k.dtype == v.dtype and act in _FLOAT_TYPES
+                and g.numel() == tokens * HV == beta.numel()
+                and (g_dtype == f32 or g_dtype == act) and (beta_dtype == f32 or beta_dtype == act)
+                and self.ss[1:] == (HV, V, K) and self.ss[0] > 0 and state.dtype in _FLOAT_TYPES
+                and K <= MAX_KEY_DIM and strides[3] == 1 and state.data_ptr() % 16 == 0
+                and not (K | strides[0] | strides[1] | strides[2]) % (16 // state.element_size())
+                and out.shape == vs and out.stride()[2:] == (V, 1) and (out.dtype == act or out.dtype == f32)
+                and device.type == "cuda" and device == k.device == v.device == g.device == beta.device
+                and device == state.device == out.device
+                and (self.a_log is None or self.plain_gating(HV)))
+
+    def plain_gating(self, HV) -> bool:
+        a_log, dt_bias, device = self.a_log, self.dt_bias, self.device
+        return (a_log.shape == dt_bias.shape == (HV,) and a_log.stride() == dt_bias.stride() == (1,)
+                and a_log.dtype in _FLOAT_TYPES and dt_bias.dtype in _FLOAT_TYPES
+                and a_log.device == device == dt_bias.device and self.softplus[0] > 0.0)
+
+    def heads_last(self, gate):
+        """A gate's token stride, heads contiguous; a copy is kept alive where its
+        shape calls for one."""
+        tokens, HV = self.vs[1], self.vs[2]
+        if gate.shape[-2:] != (tokens, HV):
+            gate = gate.reshape(tokens, HV)
+            self.keep += (gate,)
+        stride = gate.stride()
+        if HV > 1 and stride[-1] != 1:
+            fail("gate and beta heads must be contiguous")
+        return gate.data_ptr(), stride[-2]
+
     def launch(self, parts, scale, normalized) -> N.RuleLaunch:
-        enforce(_RULE_RULES, self)
+        if not self.keeps_the_rules():
+            enforce(_RULE_RULES, self)
         q, k, v, state, out = self.q, self.k, self.v, self.state, self.out
         _, tokens, heads, K = self.qs
         _, _, HV, V = self.vs
-        g, beta = self.g.reshape(tokens, HV), self.beta.reshape(tokens, HV)
-        if HV > 1 and (g.stride(1) != 1 or beta.stride(1) != 1):
-            fail("gate and beta heads must be contiguous")
+        self.keep = ()  # what the pointers below name besides the arguments
+        g, g_stride = self.heads_last(self.g)
+        beta, beta_stride = self.heads_last(self.beta)
         pages = _row_pages(parts, tokens, self.ss[0], self.device)
         gating = a_log = dt_bias = None
         if self.a_log is not None:
             a_log, dt_bias = self.a_log.data_ptr(), self.dt_bias.data_ptr()
-            self.gating = N.GatingExt(N.dtype_code(self.a_log.dtype), N.dtype_code(self.dt_bias.dtype), *self.softplus)
-            gating = ctypes.pointer(self.gating)
-        self.keep = (g, beta)  # what the pointers below name
-        strides = self.strides
+            gating = _gating_ext(self.a_log.dtype, self.dt_bias.dtype, *self.softplus)
+        strides, code = self.strides, N.dtype_code
         return N.RuleLaunch(
-            pages, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
-            state.data_ptr(), a_log, dt_bias, gating, heads, HV, K, V, q.stride(1), k.stride(1), v.stride(1),
-            g.stride(0), beta.stride(0), out.stride(1), strides[0], strides[1], strides[2], N.dtype_code(q.dtype),
-            N.dtype_code(g.dtype), N.dtype_code(beta.dtype), N.dtype_code(out.dtype), N.dtype_code(state.dtype),
-            0 if normalized else 1, K ** -0.5 if scale is None else float(scale), 0)
+            pages, q.data_ptr(), k.data_ptr(), v.data_ptr(), g, beta, out.data_ptr(), state.data_ptr(), a_log, dt_bias,
+            gating, heads, HV, K, V, q.stride(1), k.stride(1), v.stride(1), g_stride, beta_stride, out.stride(1),
+            strides[0], strides[1], strides[2], code(self.act), code(self.g.dtype), code(self.beta.dtype),
+            code(out.dtype), code(state.dtype), 0 if normalized else 1, K ** -0.5 if scale is None else float(scale), 0)
 
     def prefill(self, parts, scale, normalized):
         launch = self.launch(parts, scale, normalized)
@@ -349,6 +410,17 @@ _CONV_RULES = (
 )
 
 
+def _plain_conv(x, weight, bias, states, out) -> bool:
+    shape, taps, pages, dtype, device = x.shape, weight.shape, states.shape, x.dtype, x.device
+    return (len(shape) == len(taps) == 2 and len(pages) == 3 and 0 < shape[1] == taps[0] == pages[1]
+            and 2 <= taps[1] <= MAX_CONV_TAPS and pages[2] >= taps[1] - 1 and pages[0] > 0
+            and dtype in _FLOAT_TYPES and dtype == weight.dtype == states.dtype == out.dtype
+            and weight.is_contiguous() and x.stride(1) == 1 and out.shape == shape and out.stride(1) == 1
+            and device.type == "cuda" and device == weight.device == states.device == out.device
+            and (bias is None or (bias.shape == (shape[1],) and bias.stride(0) == 1 and bias.dtype == dtype
+                                  and bias.device == device)))
+
+
 def gdn_recoverssm_conv(
     x: torch.Tensor,
     weight: torch.Tensor,
@@ -379,8 +451,9 @@ def gdn_recoverssm_conv(
     """
     if activation not in ("silu", None):
         fail("activation must be 'silu' or None")
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-    enforce(_CONV_RULES, x, weight, bias, conv_states, out)
+    out = x.new_empty(x.shape) if out is None else out
+    if not _plain_conv(x, weight, bias, conv_states, out):
+        enforce(_CONV_RULES, x, weight, bias, conv_states, out)
     if x.numel() and out.data_ptr() == x.data_ptr():
         fail("the convolution's output may not share memory with its input")
     pages = _row_pages((query_start_loc, state_indices, final_indices, num_computed, block_table, request_indices,

@@ -81,6 +81,20 @@ class _TableCall:
         self.num_tokens = int(num_tokens)
 
 
+def _plain_tables(table, free, span, computed, lens, requests, num_tokens, block, device) -> bool:
+    """One expression that only a call keeping every rule satisfies; the rules are
+    gone through where it does not."""
+    rows = lens.shape
+    return (device.type == "cuda" and len(rows) == 1 and rows[0] <= MAX_TABLE_ROWS and num_tokens >= 0 and block > 0
+            and computed.ndim == 1 and computed.dtype in _INDEX_TYPES and lens.dtype in _INDEX_TYPES
+            and (computed.shape[0] >= rows[0] if requests is None
+                 else requests.shape == rows and requests.dtype in _INDEX_TYPES and requests.device == device)
+            and table.ndim == 2 and table.dtype == torch.int32 and table.shape[1] > 0 and table.stride(1) == 1
+            and free.ndim == 1 and free.dtype == torch.int32 and free.shape[0] > 0 and free.stride(0) == 1
+            and span.shape == (2,) and span.dtype == torch.int64 and span.stride(0) == 1
+            and device == free.device == span.device == computed.device == lens.device)
+
+
 def gdn_recoverssm_step_tables(
     block_table: torch.Tensor,
     free_pages: torch.Tensor,
@@ -114,23 +128,25 @@ def gdn_recoverssm_step_tables(
     (a buffer of its own: ``out.free_span`` must not be ``free_span``).
     ``block_table`` is filled in place.
     """
-    c = _TableCall(block_table, num_computed, query_lens, request_indices, num_tokens)
-    enforce(_TABLE_RULES, c)
-    enforce(_POOL_RULES, block_table, free_pages, free_span, block_size)
-    rows, device = query_lens.shape[0], block_table.device
-    for t in (num_computed, query_lens, request_indices):
-        if t is not None and t.device != device:
-            fail("inputs must be on the same device")
+    num_tokens, device = int(num_tokens), block_table.device
+    if not _plain_tables(block_table, free_pages, free_span, num_computed, query_lens, request_indices, num_tokens,
+                         block_size, device):
+        enforce(_TABLE_RULES, _TableCall(block_table, num_computed, query_lens, request_indices, num_tokens))
+        enforce(_POOL_RULES, block_table, free_pages, free_span, block_size)
+        for t in (num_computed, query_lens, request_indices):
+            if t is not None and t.device != device:
+                fail("inputs must be on the same device")
+    rows = query_lens.shape[0]
     if out is None:
-        out = StepTables.allocate(rows, c.num_tokens, device)
+        out = StepTables.allocate(rows, num_tokens, device)
     else:
-        _check_out(out, rows, c.num_tokens, device, free_span)
+        _check_out(out, rows, num_tokens, device, free_span)
     requests = request_indices
     launch = N.StepTablesLaunch(
         num_computed.data_ptr(), query_lens.data_ptr(), N.ptr(requests), block_table.data_ptr(),
         free_pages.data_ptr(), free_span.data_ptr(), out.free_span.data_ptr(), out.query_start_loc.data_ptr(),
         out.seq_lens.data_ptr(), out.source_indices.data_ptr(), out.final_indices.data_ptr(),
-        out.new_pages.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), rows, c.num_tokens,
+        out.new_pages.data_ptr(), out.positions.data_ptr(), out.slot_mapping.data_ptr(), rows, num_tokens,
         num_computed.shape[0], num_computed.stride(0), query_lens.stride(0),
         0 if requests is None else requests.stride(0), block_table.shape[0], block_table.shape[1],
         block_table.stride(0), free_pages.shape[0], block_size, N.dtype_code(num_computed.dtype),
