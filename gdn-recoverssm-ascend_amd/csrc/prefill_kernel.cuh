@@ -115,8 +115,9 @@ constexpr float kTUp = 0x1p10f, kTDown = 0x1p-10f;
 // 2^8 < 2^16. Other chunks are checked value by value. What F16 cannot hold at
 // all is walked token by token in FP32: chunks whose T, P or decays leave its
 // range, and columns in which four tokens' values all lie under kColumnSpan of
-// the largest (a plane's step is 2^-24), or in which a state 64 times as large
-// as any of them decays under kSteep.
+// the largest (a plane's step is 2^-24; one value of a random column does now and
+// then, four do not), or in which a state 64 times as large as any of them decays
+// under kSteep.
 constexpr float kColumnMost = 8192.0f, kColumnLeast = 256.0f, kColumnAim = 1024.0f, kColumnSpan = 0x1p-16f, kSteep = 0x1p-6f;
 
 // Row b's chunks start at slot first / 64 + b, and where they start anywhere in
@@ -820,7 +821,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
   // XCD: consecutive workgroups go to the eight XCDs in turn.
   const int wg = int(blockIdx.x), group = (wg / 8 / a.members) * 8 + wg % 8, member = wg / 8 % a.members;
   if (group >= a.pages.rows * a.H) return;
-  const int b = group / a.H, h = group % a.H;
+  const int b = row_by_length(a.pages, group / a.H), h = group % a.H;
   const int hv = h * a.ratio + member / a.slices, v0 = (member % a.slices * NW + wave) * 16;
   const Row r = load_row(a.pages, b);
   if (r.n == 0) return;
@@ -971,7 +972,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_kernel(const PrefillArgs a) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const float four = largest(0.0f, f32x4{value(t, 0), value(t, 1), value(t, 2), value(t, 3)});
-          least = least_top(least, four);
+          if (16 * t + 4 * lq + 3 < n) least = least_top(least, four);
           mv = fmaxf(mv, four);
         }
         ms = max_quarters(16.0f * ms);
@@ -1215,7 +1216,7 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
   const int lr = lane & 15;
   const int wg = int(blockIdx.x), group = (wg / 8 / a.members) * 8 + wg % 8, member = wg / 8 % a.members;
   if (group >= a.pages.rows * a.H) return;
-  const int b = group / a.H, h = group % a.H;
+  const int b = row_by_length(a.pages, group / a.H), h = group % a.H;
   const int hv = h * a.ratio + member / a.slices, v0 = member % a.slices * 16;
   const Row r = load_row(a.pages, b);
   if (r.n == 0) return;
@@ -1337,14 +1338,14 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
       };
       // As they are: sigma is the reader's. A limit below all where the chunk has to
       // be walked for what prepare found.
-      const auto publish_v = [&](const f32x2 &end_check) {
+      const auto publish_v = [&](const f32x2 &end_check, int tokens) {
         if (w == 0) {
           float most = 0.0f, least = INFINITY;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float four = largest(0.0f, f32x4{value(vv[j][0]), value(vv[j][1]), value(vv[j][2]), value(vv[j][3])});
             most = fmaxf(most, four);
-            least = least_top(least, four);
+            if (16 * j + 4 * lq + 3 < tokens) least = least_top(least, four);
           }
           most = 64.0f * max_quarters(most);
           least = 64.0f * min_quarters(least);
@@ -1354,7 +1355,7 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
       };
       load_v(n);
       load_tiles();
-      publish_v(load_check());
+      publish_v(load_check(), n);
       int in_1 = after(inside, n), n_1 = done + n < r.n ? length(done + n, in_1) : 0;
       load_v(n_1);
       load_q();
@@ -1406,7 +1407,7 @@ __global__ __launch_bounds__(kSplitThreads, split_waves(key_planes<A>(), KP)) vo
         out *= scale;
         scale = scalars(kScQ);
         lds_barrier();  // R
-        publish_v(check_next);  // of the next chunk, while there is nothing else to do
+        publish_v(check_next, n_1);  // of the next chunk, while there is nothing else to do
         load_v(n_2);
         if (check) {
           const float f = back_inside(top(top_r));

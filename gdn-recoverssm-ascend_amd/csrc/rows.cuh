@@ -102,6 +102,26 @@ __device__ __forceinline__ int last_not_above(int count, int64_t at, Key key) {
   }
 }
 
+// Row number `at` in an order by length, longest first, within each 64 rows: a
+// workgroup that walks a row alone is to start the earlier the longer it takes.
+// Whole waves.
+__device__ __forceinline__ int row_by_length(const gdn_row_pages &p, int at) {
+  if (p.rows == 1) return at;
+  const int lane = threadIdx.x & 63, base = at & ~63, row = base + lane;
+  const int count = p.rows - base < 64 ? int(p.rows - base) : 64;
+  int64_t n = -1;
+  if (lane < count)
+    n = load_index(p.query_start_loc, (row + 1) * p.qsl_stride, p.qsl_dtype) -
+        load_index(p.query_start_loc, row * p.qsl_stride, p.qsl_dtype);
+  const int length = n > 0x7fffffff ? 0x7fffffff : n < 0 ? 0 : int(n);
+  int rank = 0;
+  for (int j = 0; j < count; ++j) {
+    const int other = __builtin_amdgcn_readlane(length, j);
+    rank += (other > length) | ((other == length) & (j < lane));
+  }
+  return base + int(__builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < count && rank == at - base)));
+}
+
 // Host checks; false after set_error.
 bool check_row_pages(const char *what, const gdn_row_pages &p, int *status);
 bool check_rule(const char *what, const gdn_rule_launch *l, int *status);
