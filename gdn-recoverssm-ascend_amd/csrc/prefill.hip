@@ -9,15 +9,15 @@ namespace gdn {
 // run the chain of chunks: 256 tiles split, 1024 or 2048 at 4 or 8 waves, and a
 // round of the split scan takes about half the time of one at 4 waves. Whole
 // call, rows of 2048 tokens, BF16, K = 128, us split / 4 waves / 8 waves: 256
-// tiles 70 / 109 / 128, 512 128 / 129 / 146, 768 203 / 157 / 177, 1024 291 /
-// 193 / 209, 1280 379 / 298 / 234, 2304 665 / 483 / 435. Where two chunks'
+// tiles 72 / 122 / 148, 512 135 / 139 / 167, 768 212 / 166 / 193, 1024 296 /
+// 198 / 219, 1280 387 / 312 / 239, 2304 685 / 504 / 445. Where two chunks'
 // operands do not fit LDS, waves of scan_kernel read them from memory, each for
 // itself, split / 4 waves: BF16, K = 256, 512 tiles 199 / 674, 2048 918 / 1359;
-// FP32, K = 128, 1024 tiles 465 / 573, 2048 904 / 803; FP32, K = 256, 512 tiles
-// 734 / 1245, 1024 1428 / 1351, 2048 2804 / 1678.
-static int scan_waves(bool staged, int planes, int64_t tiles) {
+// FP32, K = 128, 1024 tiles 474 / 612, 2048 927 / 847; FP32, K = 256, 512 tiles
+// 999 / 1354, 1024 1971 / 1465, 2048 3891 / 1825.
+static int scan_waves(bool staged, int planes, int kp, int64_t tiles) {
   if (staged) return tiles <= 512 ? 0 : tiles <= 1024 ? 4 : 8;
-  return planes == 1 || tiles <= 1024 ? 0 : 4;
+  return planes == 1 || tiles <= (kp == 256 ? 768 : 1536) ? 0 : 4;
 }
 
 struct PrefillPlan {
@@ -61,7 +61,7 @@ static bool plan_prefill(const gdn_rule_launch *l, PrefillArgs &a, PrefillPlan &
   p.key_bytes = slots * H * (12 * (p.kp / 32) * p.pl) * kUnit;
   p.bytes = p.key_bytes + slots * HV * (14 + 6 * p.opl) * kUnit;
   const int64_t tiles = rp.rows * HV * ((V + 15) / 16);
-  p.nw = scan_waves(scan_staged(p.pl, p.opl, p.kp), p.pl, tiles);
+  p.nw = scan_waves(scan_staged(p.pl, p.opl, p.kp), p.pl, p.kp, tiles);
   const int per = 16 * (p.nw ? p.nw : 1);
   a.slices = int32_t((V + per - 1) / per);
   a.members = a.ratio * a.slices;

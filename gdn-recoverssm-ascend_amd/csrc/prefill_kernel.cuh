@@ -609,7 +609,7 @@ __global__ __launch_bounds__(256 * TEAMS, prepare_waves(key_planes<A>(), KP)) vo
 // what they read: operands go from memory to LDS once for all of them, a chunk
 // ahead (two buffers), without passing registers. 7777 packed tokens of 24 rows,
 // 32 value heads, K = V = 128, BF16, blocks of 256: 147 us, matrix units 18%
-// busy, vector units 29%: a wave's products wait for its own last ones, and two
+// busy, vector units 29%, and 130 us since the longest rows start first: a wave's products wait for its own last ones, and two
 // waves a SIMD are what their registers leave room for.
 // ---------------------------------------------------------------------------
 // Byte offsets of a chunk's tokens stay under kScanExtent (the host checks the
@@ -646,32 +646,52 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_buffer(const void *p, 
                                            __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
-// One token's gates and norms for the walk of a chunk token by token.
+// What the walk of a chunk, token by token, loads of a token: N fours of columns
+// of K and Q (16 columns apart), the gates as they come, one value of V.
+template <int N>
+struct WalkToken {
+  f32x4 k[N], q[N];
+  float g, beta, v;
+};
+// A pointer to device memory, said so: where the compiler does not know, its loads
+// count as LDS's too, and a barrier waits for them.
+template <typename T>
+__device__ __forceinline__ T *device_memory(T *p) {
+  return (T *)(__attribute__((address_space(1))) T *)reinterpret_cast<uintptr_t>(p);
+}
 struct Walk {
   GateParams gates;
   const PrefillArgs &a;
   int hv, h;
-  __device__ __forceinline__ Walk(const PrefillArgs &args, int hv_, int h_)
-      : gates(load_gates(args.a_log, args.dt_bias, args.gating, args.gated != 0, hv_)), a(args), hv(hv_), h(h_) {}
-  __device__ __forceinline__ float decay(int64_t tok) const {
-    return expf(log_decay(gates, load_as_f32(a.g, tok * a.g_ts + hv, a.g_dt)));
-  }
-  __device__ __forceinline__ float beta(int64_t tok) const {
-    return beta_of(gates, load_as_f32(a.beta, tok * a.beta_ts + hv, a.beta_dt));
-  }
-  __device__ __forceinline__ float norm(float sq) const { return a.l2norm ? 1.0f / sqrtf(sq + 1e-6f) : 1.0f; }
-  // Columns k0 .. k0 + 3 of a token's K or Q.
+  int64_t col;
+  bool column;
+  __device__ __forceinline__ Walk(const PrefillArgs &args, int hv_, int h_, int v)
+      : gates(load_gates(args.a_log, args.dt_bias, args.gating, args.gated != 0, hv_)), a(args), hv(hv_), h(h_),
+        col(int64_t(hv_) * args.V + (v < args.V ? v : 0)), column(v < args.V) {}
   template <typename A>
   __device__ __forceinline__ f32x4 row4(const void *p, int64_t ts, int64_t tok, int k0) const {
-    f32x4 x = {0, 0, 0, 0};
-    if (k0 < a.K) {
-      A raw[4];
-      __builtin_memcpy(raw, static_cast<const A *>(p) + tok * ts + int64_t(h) * a.K + k0, sizeof(raw));
+    const bool inside = k0 < a.K;
+    A raw[4];
+    __builtin_memcpy(raw, static_cast<const A *>(device_memory(p)) + tok * ts + int64_t(h) * a.K + (inside ? k0 : 0), sizeof(raw));
+    f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = to_f32(raw[e]);
-    }
+    for (int e = 0; e < 4; ++e) x[e] = inside ? to_f32(raw[e]) : 0.0f;
     return x;
   }
+  template <typename A, int N>
+  __device__ __forceinline__ WalkToken<N> token(int64_t tok, int k0) const {
+    WalkToken<N> t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      t.k[i] = row4<A>(a.k, a.k_ts, tok, k0 + 16 * i);
+      t.q[i] = row4<A>(a.q, a.q_ts, tok, k0 + 16 * i);
+    }
+    t.g = load_as_f32(device_memory(a.g), tok * a.g_ts + hv, a.g_dt);
+    t.beta = load_as_f32(device_memory(a.beta), tok * a.beta_ts + hv, a.beta_dt);
+    t.v = to_f32(static_cast<const A *>(device_memory(a.v))[tok * a.v_ts + col]);
+    return t;
+  }
+  __device__ __forceinline__ float norm(float sq) const { return a.l2norm ? 1.0f / sqrtf(sq + 1e-6f) : 1.0f; }
 };
 constexpr int kWalkSums = 5 * 16 * 4;  // floats: a sum, a column, a wave
 // What a token needs of the state as it stands: S k, S q, |k|^2, |q|^2, k.q.
@@ -695,14 +715,17 @@ struct WalkSums {
 // A chunk's tokens one after the other, from the inputs themselves: the state
 // (as it is, unscaled) and the outputs of this wave's 16 columns, lanes as in
 // scan_kernel. Not inlined, so that the loops around the call keep their
-// registers; the launch's arguments are read where they were passed. A token takes
-// 1.8 us, 70 times its share of a chunk: loads from memory one after the other.
+// registers; the launch's arguments are read where they were passed. A token is
+// asked for one ahead where registers allow; it takes 1.1 us in the split scan and
+// 2 in the other, some 50 times its share of a chunk.
 template <int N>
 struct WalkState {
   f32x4 s[N];
 };
 __device__ __forceinline__ const PrefillArgs &launch_arguments(const void *p) {
-  return *reinterpret_cast<const PrefillArgs *>(uniform64(int64_t(reinterpret_cast<uintptr_t>(p))));
+  // Constant memory, read through the scalar cache.
+  return *(const PrefillArgs *)(const __attribute__((address_space(4))) PrefillArgs *)uintptr_t(
+      uniform64(int64_t(reinterpret_cast<uintptr_t>(p))));
 }
 template <typename A, typename Out, int NT>
 __device__ __attribute__((noinline)) WalkState<NT> walk_chunk(WalkState<NT> state, const void *args, int first, int n,
@@ -711,26 +734,26 @@ __device__ __attribute__((noinline)) WalkState<NT> walk_chunk(WalkState<NT> stat
   first = __builtin_amdgcn_readfirstlane(first), n = __builtin_amdgcn_readfirstlane(n);
   hv = __builtin_amdgcn_readfirstlane(hv), h = __builtin_amdgcn_readfirstlane(h);
   const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-  const bool column = v0 + lr < a.V;
-  const int64_t col = int64_t(hv) * a.V + v0 + lr;
-  const Walk at(a, hv, h);
+  constexpr bool kAhead = NT <= 8;
+  const Walk at(a, hv, h, v0 + lr);
+  WalkToken<NT> token = at.token<A, NT>(first, 4 * lq);
 #pragma clang loop unroll(disable)
   for (int t = 0; t < n; ++t) {
-    const int64_t tok = first + t;
+    WalkToken<NT> next;
+    if constexpr (kAhead) next = at.token<A, NT>(first + (t + 1 < n ? t + 1 : t), 4 * lq);
     WalkSums sums;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      sums.add(state.s[i], at.row4<A>(a.k, a.k_ts, tok, 16 * i + 4 * lq), at.row4<A>(a.q, a.q_ts, tok, 16 * i + 4 * lq));
+    for (int i = 0; i < NT; ++i) sums.add(state.s[i], token.k[i], token.q[i]);
     sums.over_quarters();
-    const float d = at.decay(tok), rk = at.norm(sums.kk);
-    const float x = column ? to_f32(static_cast<const A *>(a.v)[tok * a.v_ts + col]) : 0.0f;
-    const float c = at.beta(tok) * (x - d * rk * sums.sk);
-    if (column && lq == 0)
-      static_cast<Out *>(a.out)[tok * a.out_ts + col] =
+    const float d = expf(log_decay(at.gates, token.g)), rk = at.norm(sums.kk);
+    const float c = beta_of(at.gates, token.beta) * (token.v - d * rk * sums.sk);
+    if (at.column && lq == 0)
+      static_cast<Out *>(device_memory(a.out))[(int64_t(first) + t) * a.out_ts + at.col] =
           from_f32<Out>(a.scale * at.norm(sums.qq) * fmaf(d, sums.sq, c * rk * sums.kq));
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      state.s[i] = state.s[i] * d + at.row4<A>(a.k, a.k_ts, tok, 16 * i + 4 * lq) * (c * rk);
+    for (int i = 0; i < NT; ++i) state.s[i] = state.s[i] * d + token.k[i] * (c * rk);
+    if constexpr (!kAhead) next = at.token<A, NT>(first + (t + 1 < n ? t + 1 : t), 4 * lq);
+    token = next;
   }
   return state;
 }
@@ -744,21 +767,15 @@ __device__ __attribute__((noinline)) WalkState<KT> walk_chunk_split(WalkState<KT
   first = __builtin_amdgcn_readfirstlane(first), n = __builtin_amdgcn_readfirstlane(n);
   hv = __builtin_amdgcn_readfirstlane(hv), h = __builtin_amdgcn_readfirstlane(h);
   const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const bool column = v0 + lr < a.V;
-  const int64_t col = int64_t(hv) * a.V + v0 + lr;
-  const Walk at(a, hv, h);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), k0 = 16 * w * KT + 4 * lq;
+  const Walk at(a, hv, h, v0 + lr);
+  WalkToken<KT> token = at.token<A, KT>(first, k0);
 #pragma clang loop unroll(disable)
   for (int t = 0; t < n; ++t) {
-    const int64_t tok = first + t;
-    f32x4 k[KT];
+    const WalkToken<KT> next = at.token<A, KT>(first + (t + 1 < n ? t + 1 : t), k0);
     WalkSums own;
 #pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      const int k0 = 16 * (w * KT + i) + 4 * lq;
-      k[i] = at.row4<A>(a.k, a.k_ts, tok, k0);
-      own.add(state.s[i], k[i], at.row4<A>(a.q, a.q_ts, tok, k0));
-    }
+    for (int i = 0; i < KT; ++i) own.add(state.s[i], token.k[i], token.q[i]);
     own.over_quarters();
     // Two sets: a wave is at most one token ahead of the slowest.
     float *const sums = sums_of + (t & 1) * kWalkSums + lr * 4;
@@ -771,14 +788,14 @@ __device__ __attribute__((noinline)) WalkState<KT> walk_chunk_split(WalkState<KT
       const f32x4 x = *reinterpret_cast<const f32x4 *>(sums + 64 * i);
       return (x[0] + x[1]) + (x[2] + x[3]);
     };
-    const float d = at.decay(tok), rk = at.norm(total(2));
-    const float x = column ? to_f32(static_cast<const A *>(a.v)[tok * a.v_ts + col]) : 0.0f;
-    const float c = at.beta(tok) * (x - d * rk * total(0));
-    if (column && lq == 0 && w == 0)
-      static_cast<Out *>(a.out)[tok * a.out_ts + col] =
+    const float d = expf(log_decay(at.gates, token.g)), rk = at.norm(total(2));
+    const float c = beta_of(at.gates, token.beta) * (token.v - d * rk * total(0));
+    if (at.column && lq == 0 && w == 0)
+      static_cast<Out *>(device_memory(a.out))[(int64_t(first) + t) * a.out_ts + at.col] =
           from_f32<Out>(a.scale * at.norm(total(3)) * fmaf(d, total(1), c * rk * total(4)));
 #pragma unroll
-    for (int i = 0; i < KT; ++i) state.s[i] = state.s[i] * d + k[i] * (c * rk);
+    for (int i = 0; i < KT; ++i) state.s[i] = state.s[i] * d + token.k[i] * (c * rk);
+    token = next;
   }
   return state;
 }

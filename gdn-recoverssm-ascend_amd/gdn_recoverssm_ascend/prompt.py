@@ -280,7 +280,7 @@ def gdn_recoverssm_prefill(
     tokens before it in its own row (the chunk), besides those after it. Chunks
     whose values a matrix core's operands cannot hold (decays that grow, keys far
     from unit length, columns that fall by a factor of 2^16 within 64 tokens) are
-    computed token by token, some 70 times as slowly.
+    computed token by token, some 50 times as slowly.
 
     Token strides of ``v`` and ``out`` must be at least the value dim and span
     under 1 GiB per 64 tokens. Working memory is taken from torch's allocator:
